@@ -155,9 +155,12 @@ template <> struct Elem<double> {
 // 16-byte store of data that nothing on the GPU reads again soon: non-temporal AND system scope.
 // The compiler's non-temporal store sets only the first of the two; with both the (R,V) gradient
 // stream runs about 3 % faster on MI355X (395 -> 383 us for 1.28 GB read + 1.28 GB written).
+// A store of more than 8 bytes reads its data registers while the next instructions issue: a vector
+// instruction may overwrite them only two wait states later.  The compiler keeps that distance for
+// the stores it emits itself but does not look into inline assembly, so the wait is part of it.
 typedef int v4i_store_t __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void store_streaming_16(void* p, v4i_store_t v) {
-    asm volatile("global_store_dwordx4 %0, %1, off sc1 nt" : : "v"(p), "v"(v) : "memory");
+    asm volatile("global_store_dwordx4 %0, %1, off sc1 nt\n\ts_nop 1" : : "v"(p), "v"(v) : "memory");
 }
 
 template <typename T, int VEC> struct alignas(sizeof(T) * VEC) PackT { T e[VEC]; };
