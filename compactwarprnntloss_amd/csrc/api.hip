@@ -173,7 +173,7 @@ using namespace cwr;
 
 extern "C" {
 
-int cwr_version(void) { return 130; }
+int cwr_version(void) { return 140; }
 
 const char* cwr_strerror(int status) {
     switch (status) {
@@ -574,6 +574,92 @@ int cwr_join_backward(const void* dh, const void* h, int dtype, int act, int64_t
     if (misaligned(dh, es) || misaligned(h, es) || misaligned(df, es) || misaligned(dg, es)) return CWR_ERR_ALIGN;
     return launch_join(dtype, act, true, dh, h, df, dg, lx, ly, reinterpret_cast<const i64*>(row_off), N, T_pad,
                        Up_pad, H, R, nullptr, static_cast<hipStream_t>(stream));
+}
+
+// What the calls on rows of logits share.
+static int check_rows(const void* x, int dtype, int64_t R, int64_t V, int64_t x_stride, int64_t K, double temperature) {
+    if (dtype < CWR_F32 || dtype > CWR_F64) return CWR_ERR_DTYPE;
+    if (R < 0 || V < 1 || x_stride < 0 || K < 0) return CWR_ERR_SHAPE;
+    if (V > 0x3fffffff) return CWR_ERR_TOO_LARGE;
+    if (K > CWR_MAX_ROW_TOKENS) return CWR_ERR_TOO_LARGE;
+    if (!(temperature > 0.0) || !(temperature <= 1e30) || temperature < 1e-30) return CWR_ERR_SHAPE;
+    if (R > 0 && !x) return CWR_ERR_NULL;
+    if (misaligned(x, elem_size(dtype))) return CWR_ERR_ALIGN;
+    return CWR_OK;
+}
+
+static int check_scores(int64_t R, int64_t V, const int32_t* tokens, int64_t M, int64_t K) {
+    if (M < 0 || K > V) return CWR_ERR_SHAPE;
+    if (M > CWR_MAX_ROW_TOKENS) return CWR_ERR_TOO_LARGE;
+    if (R > 0 && M > 0 && !tokens) return CWR_ERR_NULL;
+    return misaligned(tokens, 4) ? CWR_ERR_ALIGN : CWR_OK;
+}
+
+int cwr_token_logprobs(const void* x, int dtype, int64_t R, int64_t V, int64_t x_stride, const int32_t* tokens,
+                       int64_t M, int64_t K, double temperature, float* stat, float* logprobs, float* entropy,
+                       float* lse, float* top_logprobs, int32_t* top_index, int32_t* status, void* stream) {
+    int rc = check_rows(x, dtype, R, V, x_stride, K, temperature);
+    if (rc == CWR_OK) rc = check_scores(R, V, tokens, M, K);
+    if (rc != CWR_OK) return rc;
+    if (R > 0 && ((M > 0 && !logprobs) || (K > 0 && (!top_logprobs || !top_index)))) return CWR_ERR_NULL;
+    if (misaligned(stat, 8) || misaligned(logprobs, 4) || misaligned(entropy, 4) || misaligned(lse, 4) ||
+        misaligned(top_logprobs, 4) || misaligned(top_index, 4) || misaligned(status, 4))
+        return CWR_ERR_ALIGN;
+    const RowScores s = {tokens, M, K, stat, logprobs, entropy, lse, top_logprobs, top_index, status};
+    return launch_scores(x, dtype, R, V, x_stride, temperature, s, static_cast<hipStream_t>(stream));
+}
+
+int cwr_token_logprobs_backward(const void* x, int dtype, int64_t R, int64_t V, int64_t x_stride,
+                                const int32_t* tokens, int64_t M, const int32_t* top_index, int64_t K,
+                                double temperature, const float* stat, const float* entropy, const float* g_logprobs,
+                                const float* g_entropy, const float* g_lse, const float* g_top, void* dx, void* stream) {
+    int rc = check_rows(x, dtype, R, V, x_stride, K, temperature);
+    if (rc == CWR_OK) rc = check_scores(R, V, tokens, M, K);
+    if (rc != CWR_OK) return rc;
+    if (R > 0 && (!stat || !dx || (K > 0 && !top_index) || (g_entropy && !entropy))) return CWR_ERR_NULL;
+    if (misaligned(stat, 8) || misaligned(entropy, 4) || misaligned(g_logprobs, 4) || misaligned(g_entropy, 4) ||
+        misaligned(g_lse, 4) || misaligned(g_top, 4) || misaligned(top_index, 4) || misaligned(dx, elem_size(dtype)))
+        return CWR_ERR_ALIGN;
+    const RowScoreGrads s = {stat, entropy, tokens, top_index, M, K, g_logprobs, g_entropy, g_lse, g_top};
+    return launch_scores_grad(x, dtype, R, V, x_stride, temperature, s, dx, static_cast<hipStream_t>(stream));
+}
+
+size_t cwr_distill_workspace_bytes(void) { return sum_workspace_bytes(); }
+
+static int check_distill(int64_t R, const float* top, const int32_t* top_index, int64_t K, int tail) {
+    if (K < 1) return CWR_ERR_SHAPE;
+    if (tail != 0 && tail != 1) return CWR_ERR_MODE;
+    if (R > 0 && (!top || !top_index)) return CWR_ERR_NULL;
+    return misaligned(top, 4) || misaligned(top_index, 4) ? CWR_ERR_ALIGN : CWR_OK;
+}
+
+int cwr_distill(const void* x, int dtype, int64_t R, int64_t V, int64_t x_stride, const float* top,
+                const int32_t* top_index, int64_t K, double temperature, int tail, float* loss, float* stat,
+                float* reduced, void* workspace, int32_t* status, void* stream) {
+    int rc = check_rows(x, dtype, R, V, x_stride, K, temperature);
+    if (rc == CWR_OK) rc = check_distill(R, top, top_index, K, tail);
+    if (rc != CWR_OK) return rc;
+    if ((R > 0 && !loss) || (reduced && !workspace)) return CWR_ERR_NULL;
+    if (misaligned(loss, 4) || misaligned(stat, 16) || misaligned(reduced, 4) || misaligned(workspace, 8) ||
+        misaligned(status, 4))
+        return CWR_ERR_ALIGN;
+    const RowDistill s = {top, top_index, K, tail != 0, stat};
+    return launch_distill(x, dtype, R, V, x_stride, temperature, s, loss, reduced, workspace, status,
+                          static_cast<hipStream_t>(stream));
+}
+
+int cwr_distill_backward(const void* x, int dtype, int64_t R, int64_t V, int64_t x_stride, const float* top,
+                         const int32_t* top_index, int64_t K, double temperature, int tail, const float* stat,
+                         const float* grad_loss, int64_t grad_stride, float grad_scale, void* dx, void* stream) {
+    int rc = check_rows(x, dtype, R, V, x_stride, K, temperature);
+    if (rc == CWR_OK) rc = check_distill(R, top, top_index, K, tail);
+    if (rc != CWR_OK) return rc;
+    if (grad_stride != 0 && grad_stride != 1) return CWR_ERR_SHAPE;
+    if (R > 0 && (!stat || !grad_loss || !dx)) return CWR_ERR_NULL;
+    if (misaligned(stat, 16) || misaligned(grad_loss, 4) || misaligned(dx, elem_size(dtype))) return CWR_ERR_ALIGN;
+    const RowDistill s = {top, top_index, K, tail != 0, const_cast<float*>(stat)};
+    const GradOut go = {grad_loss, grad_stride, grad_scale};
+    return launch_distill_grad(x, dtype, R, V, x_stride, temperature, s, go, dx, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

@@ -109,6 +109,48 @@ int launch_join(int dtype, int act, bool backward, const void* a, const void* b,
                 const int* ly, const i64* row_off, i64 N, i64 T_pad, i64 Up_pad, i64 H, i64 R, int* status,
                 hipStream_t stream);
 
+// Scores of rows of logits (scores.hip): pointers as in cwr_token_logprobs / cwr_token_logprobs_backward
+struct RowScores {
+    const int* tokens;
+    i64 M, K;
+    float* stat;
+    float* logprobs;
+    float* entropy;
+    float* lse;
+    float* top_logprobs;
+    int* top_index;
+    int* status;
+};
+struct RowScoreGrads {
+    const float* stat;
+    const float* entropy;
+    const int* tokens;
+    const int* top_index;
+    i64 M, K;
+    const float* g_logprobs;
+    const float* g_entropy;
+    const float* g_lse;
+    const float* g_top;
+};
+int launch_scores(const void* x, int dtype, i64 R, i64 V, i64 stride, double temperature, const RowScores& s,
+                  hipStream_t stream);
+int launch_scores_grad(const void* x, int dtype, i64 R, i64 V, i64 stride, double temperature, const RowScoreGrads& s,
+                       void* dx, hipStream_t stream);
+
+// Distillation of rows of logits (distill.hip): pointers as in cwr_distill / cwr_distill_backward
+struct RowDistill {
+    const float* top;
+    const int* index;
+    i64 K;
+    bool tail;
+    float* stat;  // (R, 4)
+};
+size_t sum_workspace_bytes();
+int launch_distill(const void* x, int dtype, i64 R, i64 V, i64 stride, double temperature, const RowDistill& s,
+                   float* loss, float* reduced, void* workspace, int* status, hipStream_t stream);
+int launch_distill_grad(const void* x, int dtype, i64 R, i64 V, i64 stride, double temperature, const RowDistill& s,
+                        const GradOut go, void* dx, hipStream_t stream);
+
 // Launches go through CWR_LAUNCH, which first drops whatever error an earlier HIP call of this thread
 // (the caller's, or another library's) left pending, so that check_launch() reports this launch and
 // nothing else.  The runtime's own code is kept for cwr_strerror.

@@ -1,0 +1,224 @@
+// What the row kernels of scores.hip and distill.hip share: a row of V logits cut into 16-byte packs,
+// 16 elements per lane and chunk, and the cross-lane reductions over the lanes that share a row.
+//
+// A chunk is 16 G elements held by G consecutive lanes: pack i of lane l covers elements
+// ((i G + l) VEC - off) .. + VEC, so that the lanes of one load instruction touch consecutive
+// 16-byte packs.  `off` shifts the packs of a row that does not start on a 16-byte boundary back to
+// that grid; the packs at its two ends, which then stick out of the row, are read element by element
+// and never touch memory outside the row.
+#pragma once
+
+#include "cwr_device.hpp"
+#include "cwr_pack.hpp"
+
+namespace cwr {
+
+typedef unsigned long long u64;
+
+constexpr int kLaneElems = 16;  // elements a lane holds of a chunk
+
+// How a softmax at temperature T is evaluated: exponents in bits, t = x * c with c = log2(e) / T.
+struct Temper {
+    float c;     // log2(e) / T
+    double inv;  // 1 / T
+};
+
+template <typename T> struct RowPacks {
+    static constexpr int VEC = Elem<T>::VEC;
+    static constexpr int NP = kLaneElems / VEC;  // packs a lane holds
+};
+
+// elements in front of the first 16-byte boundary grid point at or before p
+template <typename T> __device__ __forceinline__ int grid_offset(const T* p) {
+    return (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
+}
+
+// The pack of row elements [e, e + VEC); elements outside [0, V) come back as -inf.  EDGE = false: rows
+// are whole packs on the 16-byte grid, a pack is inside the row or outside it.
+template <typename T, bool EDGE, bool NT>
+__device__ __forceinline__ v4i load_pack(const T* __restrict__ row, int e, int V) {
+    constexpr int VEC = Elem<T>::VEC;
+    if (!EDGE) {
+        v4i r = Pack<T>::neg_inf();
+        if (e < V) r = load_raw<NT>(row + e);
+        return r;
+    }
+    // a row off the element grid of 16 bytes: the hardware takes any element-aligned address
+    typedef v4i v4i_any __attribute__((aligned(2)));
+    if (e >= 0 && e + VEC <= V) return *reinterpret_cast<const v4i_any*>(row + e);
+    PackT<T, VEC> p;
+    const v4i none = Pack<T>::neg_inf();
+    __builtin_memcpy(&p, &none, 16);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+        if ((unsigned)(e + j) < (unsigned)V) p.e[j] = row[e + j];
+    v4i r;
+    __builtin_memcpy(&r, &p, 16);
+    return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack_chunk(const v4i (&raw)[RowPacks<T>::NP], float (&v)[kLaneElems]) {
+    constexpr int VEC = RowPacks<T>::VEC;
+#pragma unroll
+    for (int i = 0; i < RowPacks<T>::NP; ++i) {
+        float t[VEC];
+        Pack<T>::unpack(raw[i], t);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[i * VEC + j] = t[j];
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// reductions over aligned groups of W lanes
+// ---------------------------------------------------------------------------------------------
+struct OpMaxI { static __device__ __forceinline__ int apply(int a, int b) { return a > b ? a : b; } };
+struct OpMinI { static __device__ __forceinline__ int apply(int a, int b) { return a < b ? a : b; } };
+
+template <int W, class Op>
+__device__ __forceinline__ int group_allreduce_i32(int v) {
+    if (W >= 2) v = Op::apply(v, dpp_i32<DPP_QUAD_XOR1>(v, v));
+    if (W >= 4) v = Op::apply(v, dpp_i32<DPP_QUAD_XOR2>(v, v));
+    if (W >= 8) v = Op::apply(v, dpp_i32<DPP_ROW_HALF_MIRROR>(v, v));
+    if (W >= 16) v = Op::apply(v, dpp_i32<DPP_ROW_MIRROR>(v, v));
+    if (W >= 32) v = Op::apply(v, __shfl_xor(v, 16));
+    if (W >= 64) v = Op::apply(v, __shfl_xor(v, 32));
+    return v;
+}
+
+template <int W> __device__ __forceinline__ double group_sum_f64(double v) {
+#pragma unroll
+    for (int d = 1; d < W; d <<= 1) v += __shfl_xor(v, d);
+    return v;
+}
+
+// Orders what the lanes of one wave write to LDS before what its other lanes read there.  A wave's LDS
+// accesses are performed in order; this keeps the compiler from moving them.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// ---------------------------------------------------------------------------------------------
+// running softmax statistics of a row, in bits
+// ---------------------------------------------------------------------------------------------
+// s = sum of 2^t and u = sum of 2^t t over the elements seen, t = x c - m c, m the largest x seen
+// (-inf: none seen, or nothing but -inf; s and u are then 0).  m is the same in all lanes of the row.
+struct Online {
+    float m, s, u;
+};
+
+// What elements are measured against: t = fma(x - sub, c, -ms).  Normally sub = 0 and ms = m c rounded to
+// fp32: one fma per element, and what the rounding loses is the same for the whole row and comes back
+// exactly from an fma (ms_slip).  Where m c is out of all proportion (rows masked with the lowest
+// value of their type) that product would overflow, and m is subtracted first.
+struct Anchor {
+    float sub, ms;
+};
+__device__ __forceinline__ bool far_off(float m, float c) { return !(fabsf(m * c) < 0x1p100f); }  // NaN, inf too
+__device__ __forceinline__ Anchor anchor(float m, float c) {
+    Anchor a = {0.f, m * c};
+    if (far_off(m, c)) {
+        a.sub = m;
+        a.ms = 0.f;
+    }
+    if (m == -INFINITY) a.sub = 0.f;  // nothing but -inf: t = -inf
+    return a;
+}
+__device__ __forceinline__ float measure(float x, const Anchor& a, float c) { return fmaf(x - a.sub, c, -a.ms); }
+__device__ __forceinline__ float ms_slip(float m, float c) {  // m c - ms
+    return far_off(m, c) ? 0.f : fmaf(m, c, -(m * c));
+}
+// how far, in bits, what is measured against `from` lies below what is measured against `to` >= from
+__device__ __forceinline__ float anchor_shift(float from, float to, float c) {
+    if (from == to) return 0.f;
+    return far_off(from, c) || far_off(to, c) ? -INFINITY : from * c - to * c;
+}
+
+constexpr float kTFloor = -1024.f;  // 2^t is 0 far above it; keeps 0 * t finite where x is -inf
+
+// the rare rows whose anchor has something to subtract first
+template <int N> __device__ __forceinline__ void subtract_far(float (&v)[N], const Anchor& a) {
+    if (__ballot(a.sub != 0.f) != 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] -= a.sub;
+    }
+}
+
+template <bool ENTROPY>
+__device__ __forceinline__ void online_chunk(const float (&x)[kLaneElems], float m, float c, float& s, float& u) {
+    const Anchor a = anchor(m, c);
+    float v[kLaneElems];
+#pragma unroll
+    for (int i = 0; i < kLaneElems; ++i) v[i] = x[i];
+    subtract_far(v, a);
+    float sa = 0.f, sb = 0.f, ua = 0.f, ub = 0.f;
+#pragma unroll
+    for (int i = 0; i < kLaneElems; i += 2) {
+        const float t0 = fmaf(v[i], c, -a.ms), t1 = fmaf(v[i + 1], c, -a.ms);
+        const float e0 = fast_exp2(t0), e1 = fast_exp2(t1);
+        sa += e0;
+        sb += e1;
+        if (ENTROPY) {
+            ua = fmaf(e0, fmaxf(t0, kTFloor), ua);
+            ub = fmaf(e1, fmaxf(t1, kTFloor), ub);
+        }
+    }
+    s = sa + sb;
+    u = ua + ub;
+}
+
+// state o measured against a maximum mn at least as large
+__device__ __forceinline__ void online_rebase(Online& o, float mn, float c) {
+    if (o.m != mn) {
+        const float d = fmaxf(anchor_shift(o.m, mn, c), kTFloor);
+        const float f = fast_exp2(d);
+        o.u = f * fmaf(o.s, d, o.u);
+        o.s *= f;
+        o.m = mn;
+    }
+}
+
+__device__ __forceinline__ float chunk_max(const float (&v)[kLaneElems]) {
+    float m = v[0];
+#pragma unroll
+    for (int i = 1; i < kLaneElems; ++i) m = fmaxf(m, v[i]);
+    return m;
+}
+
+// log2 of the sum of 2^((x - m) c) from the sum s of 2^(x c - ms)
+__device__ __forceinline__ float log2_sum(const Online& o, float c) { return log2_of_sum(o.s) - ms_slip(o.m, c); }
+
+// ln p of the logit x in a row with maximum m and log2 sum l2.  The difference x - m is exact in 64 bits and
+// the logarithm of the sum is small in a peaked row: the result keeps its absolute accuracy however
+// large the logits are.  A row of nothing but -inf gives -inf.
+__device__ __forceinline__ float logprob(float x, float m, float l2, const Temper& tp) {
+    if (x == -INFINITY && !(l2 != l2)) return -INFINITY;
+    return (float)(((double)x - (double)m) * tp.inv - (double)l2 * 0.6931471805599453);
+}
+
+// ---------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------
+inline unsigned wave_blocks(i64 waves) {  // whole workgroups, a multiple of the XCDs
+    return (unsigned)(((waves + kWavesPerBlock - 1) / kWavesPerBlock + 7) & ~(i64)7);
+}
+
+// rows of V elements, `stride` apart, are whole packs on the 16-byte grid
+template <typename T> inline bool on_grid(const void* p, i64 stride, int V) {
+    constexpr int VEC = Elem<T>::VEC;
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && V % VEC == 0 && stride % VEC == 0;
+}
+
+// Waves that share a row of `chunks` chunks: enough of them to fill 1024 SIMDs when there are few rows, as
+// long as each has a chunk of its own.
+inline int row_waves(i64 R, i64 chunks) { return chunks >= 16 && R < 1024 ? 16 : chunks >= 4 && R < 16384 ? 4 : 1; }
+
+inline Temper make_temper(double temperature) {
+    Temper tp;
+    tp.c = (float)(1.4426950408889634 / temperature);
+    tp.inv = 1.0 / temperature;
+    return tp;
+}
+
+}  // namespace cwr

@@ -335,6 +335,68 @@ int cwr_joint_backward(const void* h, const void* w, const float* bias, int dtyp
                        int64_t N, int32_t blank, const int32_t* rowinfo, const float* grads, const float* lse,
                        const float* grad_costs, int64_t grad_stride, float grad_scale, void* dlogits, void* stream);
 
+/* Scores of rows of logits, each row on its own: with z = x[r, :] / temperature, lse = log sum exp z and
+ * p = exp(z - lse),
+ *   logprobs[r, j]      = log p[tokens[r, j]] for M given tokens;  a token of -1 stands for none (0); one
+ *                         outside [0, V) gives NaN and raises CWR_FLAG_BAD_LABEL in status
+ *   entropy[r]          = -sum p log p,   lse[r] = lse
+ *   top_index[r, k], top_logprobs[r, k], k < K: the K largest entries in descending order, equal ones by
+ *                         ascending index (-0 equals +0, NaN ranks with -inf)
+ * One read of x.  The reference has no counterpart: its callers run log_softmax on stored logits
+ * (test/test.py:19-20).  The compact rows of a lattice are scored with tokens (blank, label).
+ *   x            (R, V) of any cwr_dtype (64-bit entries are rounded to fp32 when read, as everywhere in
+ *                this library), row r at x + r * x_stride, entries of a row adjacent; x_stride >= 0
+ *   tokens       (R, M) int32, M <= 64;  K <= 64, K <= V;  temperature > 0 and finite
+ *   stat         (R, 2) fp32 for cwr_token_logprobs_backward: row maximum, log2 of the scaled sum;  NULL: not kept
+ *   logprobs     (R, M) fp32, NULL only if M = 0;  entropy, lse (R) fp32, each may be NULL
+ *   top_logprobs (R, K) fp32 and top_index (R, K) int32, NULL only if K = 0
+ *   status       4 x int32 the caller has zeroed, or NULL
+ * A row of nothing but -inf: lse = -inf, log-probabilities -inf, entropy 0, gradient 0.  A row with NaN or
+ * +inf in it: everything but top_index is NaN. */
+#define CWR_MAX_ROW_TOKENS 64
+int cwr_token_logprobs(const void* x, int dtype, int64_t R, int64_t V, int64_t x_stride, const int32_t* tokens,
+                       int64_t M, int64_t K, double temperature, float* stat, float* logprobs, float* entropy,
+                       float* lse, float* top_logprobs, int32_t* top_index, int32_t* status, void* stream);
+
+/* Backward of cwr_token_logprobs: dx (R, V) of `dtype`, contiguous, every element written.  g_logprobs
+ * (R, M), g_entropy (R), g_lse (R), g_top (R, K) fp32 are the gradients of its outputs, each may be NULL
+ * (zero); tokens of -1 or outside [0, V) get none.  stat, entropy (needed with g_entropy) and top_index
+ * as that call wrote them; all other arguments as there. */
+int cwr_token_logprobs_backward(const void* x, int dtype, int64_t R, int64_t V, int64_t x_stride,
+                                const int32_t* tokens, int64_t M, const int32_t* top_index, int64_t K,
+                                double temperature, const float* stat, const float* entropy, const float* g_logprobs,
+                                const float* g_entropy, const float* g_lse, const float* g_top, void* dx, void* stream);
+
+/* Distillation of rows of logits from a teacher's top logits.  z = x[r, :] / temperature, p = softmax(z);
+ * the teacher's entry k of row r is index top_index[r, k] with value top[r, k]; an index of -1 is absent.
+ *   tail = 0: q = softmax of the row's values / temperature,
+ *             loss[r] = temperature^2 * sum_k q_k (log q_k - log p[i_k])
+ *   tail = 1: values are log-probabilities at this temperature, q_k = exp(value).  What they leave,
+ *             q_r = max(0, 1 - sum q), is one more class, and so is the mass p_r the student gives to entries
+ *             not listed:  loss[r] = temperature^2 * (sum_k q_k (log q_k - log p[i_k]) + q_r (log q_r - log p_r)).
+ *             A row whose unlisted entries are none, or all -inf, has no such class (no q_r term).
+ * With the list (blank, label) and a tail this is the three-class distillation of a lattice cell.
+ * A row whose list is empty (all absent) has loss 0 and gradient 0.  An index listed twice counts each
+ * time, and once for what is not listed.  An index below -1 or >= V: loss NaN, gradient 0,
+ * CWR_FLAG_BAD_LABEL.  The reference has no counterpart.
+ *   x, dtype, x_stride, temperature, status as for cwr_token_logprobs
+ *   top (R, K) fp32, top_index (R, K) int32, 1 <= K <= 64
+ *   loss (R) fp32;  stat (R, 4) fp32, 16-byte aligned, for cwr_distill_backward, NULL: not kept
+ *   reduced      NULL, or 2 x fp32: sum and mean of the losses, added in 64 bits in a fixed order; needs
+ *                workspace of cwr_distill_workspace_bytes() bytes, 8-byte aligned (else NULL) */
+size_t cwr_distill_workspace_bytes(void);
+int cwr_distill(const void* x, int dtype, int64_t R, int64_t V, int64_t x_stride, const float* top,
+                const int32_t* top_index, int64_t K, double temperature, int tail, float* loss, float* stat,
+                float* reduced, void* workspace, int32_t* status, void* stream);
+
+/* Backward of cwr_distill: dx (R, V) of `dtype`, contiguous, every element written.
+ *   dx[r, v] = g T (p[v] Q - sum_{k: i_k = v} q_k - [v not listed] q_r p[v] / p_r),   Q = sum q (+ q_r),
+ * g = grad_loss[r * grad_stride] * grad_scale (grad_stride 1 or 0, as for cwr_backward); stat as
+ * cwr_distill wrote it, all other arguments as there. */
+int cwr_distill_backward(const void* x, int dtype, int64_t R, int64_t V, int64_t x_stride, const float* top,
+                         const int32_t* top_index, int64_t K, double temperature, int tail, const float* stat,
+                         const float* grad_loss, int64_t grad_stride, float grad_scale, void* dx, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
