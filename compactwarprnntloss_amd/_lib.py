@@ -66,9 +66,13 @@ SIGNATURES = {
     "cwr_token_logprobs": (C.c_int, [_p, C.c_int, _i64, _i64, _i64, _p, _i64, _i64, C.c_double, _p, _p, _p, _p, _p, _p,
                                      _p, _p]),
     "cwr_token_logprobs_backward": (C.c_int, [_p, C.c_int, _i64, _i64, _i64, _p, _i64, _p, _i64, C.c_double, _p, _p, _p,
-                                              _p, _p, _p, _p, _p]),
+                                              _p, _p, _p, _p]),
+    "cwr_joint_token_logprobs_workspace_bytes": (_sz, [_i64, _i64]),
+    "cwr_joint_token_logprobs": (C.c_int, [_p, _p, _p, C.c_int, C.c_int, _i64, _i64, _i64, _p, _i64, _i64, C.c_double,
+                                           _p, _p, _p, _p, _p, _p, _sz, _p, _p]),
     "cwr_distill_workspace_bytes": (_sz, []),
-    "cwr_distill": (C.c_int, [_p, C.c_int, _i64, _i64, _i64, _p, _p, _i64, C.c_double, C.c_int, _p, _p, _p, _p, _p, _p]),
+    "cwr_distill": (C.c_int, [_p, C.c_int, _i64, _i64, _i64, _p, _p, _i64, C.c_double, C.c_int, _p, _p, _p, _p, _p, _p,
+                              _p]),
     "cwr_distill_backward": (C.c_int, [_p, C.c_int, _i64, _i64, _i64, _p, _p, _i64, C.c_double, C.c_int, _p, _p, _i64,
                                        C.c_float, _p, _p]),
     "cwr_join": (C.c_int, [_p, _p, C.c_int, C.c_int, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _p, _p, _p]),

@@ -602,7 +602,7 @@ int cwr_token_logprobs(const void* x, int dtype, int64_t R, int64_t V, int64_t x
     if (rc == CWR_OK) rc = check_scores(R, V, tokens, M, K);
     if (rc != CWR_OK) return rc;
     if (R > 0 && ((M > 0 && !logprobs) || (K > 0 && (!top_logprobs || !top_index)))) return CWR_ERR_NULL;
-    if (misaligned(stat, 8) || misaligned(logprobs, 4) || misaligned(entropy, 4) || misaligned(lse, 4) ||
+    if (misaligned(stat, 16) || misaligned(logprobs, 4) || misaligned(entropy, 4) || misaligned(lse, 4) ||
         misaligned(top_logprobs, 4) || misaligned(top_index, 4) || misaligned(status, 4))
         return CWR_ERR_ALIGN;
     const RowScores s = {tokens, M, K, stat, logprobs, entropy, lse, top_logprobs, top_index, status};
@@ -611,17 +611,43 @@ int cwr_token_logprobs(const void* x, int dtype, int64_t R, int64_t V, int64_t x
 
 int cwr_token_logprobs_backward(const void* x, int dtype, int64_t R, int64_t V, int64_t x_stride,
                                 const int32_t* tokens, int64_t M, const int32_t* top_index, int64_t K,
-                                double temperature, const float* stat, const float* entropy, const float* g_logprobs,
-                                const float* g_entropy, const float* g_lse, const float* g_top, void* dx, void* stream) {
+                                double temperature, const float* stat, const float* g_logprobs, const float* g_entropy,
+                                const float* g_lse, const float* g_top, void* dx, void* stream) {
     int rc = check_rows(x, dtype, R, V, x_stride, K, temperature);
     if (rc == CWR_OK) rc = check_scores(R, V, tokens, M, K);
     if (rc != CWR_OK) return rc;
-    if (R > 0 && (!stat || !dx || (K > 0 && !top_index) || (g_entropy && !entropy))) return CWR_ERR_NULL;
-    if (misaligned(stat, 8) || misaligned(entropy, 4) || misaligned(g_logprobs, 4) || misaligned(g_entropy, 4) ||
-        misaligned(g_lse, 4) || misaligned(g_top, 4) || misaligned(top_index, 4) || misaligned(dx, elem_size(dtype)))
+    if (R > 0 && (!stat || !dx || (K > 0 && !top_index))) return CWR_ERR_NULL;
+    if (misaligned(stat, 16) || misaligned(g_logprobs, 4) || misaligned(g_entropy, 4) || misaligned(g_lse, 4) || misaligned(g_top, 4) || misaligned(top_index, 4) || misaligned(dx, elem_size(dtype)))
         return CWR_ERR_ALIGN;
-    const RowScoreGrads s = {stat, entropy, tokens, top_index, M, K, g_logprobs, g_entropy, g_lse, g_top};
+    const RowScoreGrads s = {stat, tokens, top_index, M, K, g_logprobs, g_entropy, g_lse, g_top};
     return launch_scores_grad(x, dtype, R, V, x_stride, temperature, s, dx, static_cast<hipStream_t>(stream));
+}
+
+size_t cwr_joint_token_logprobs_workspace_bytes(int64_t R, int64_t V) {
+    if (R < 0 || V < 1 || V > 0x3fffffff) return 0;
+    return joint_scores_workspace_bytes(R, V);
+}
+
+int cwr_joint_token_logprobs(const void* h, const void* w, const void* bias, int bias_dtype, int dtype, int64_t R,
+                             int64_t H, int64_t V, const int32_t* tokens, int64_t M, int64_t K, double temperature,
+                             float* logprobs, float* entropy, float* lse, float* top_logprobs, int32_t* top_index,
+                             void* workspace, size_t workspace_bytes_, int32_t* status, void* stream) {
+    if (dtype != CWR_F16 && dtype != CWR_BF16) return CWR_ERR_DTYPE;
+    if (bias && bias_dtype != CWR_F32 && bias_dtype != dtype) return CWR_ERR_DTYPE;
+    int rc = check_rows(h, dtype, R, V, 0, K, temperature);
+    if (rc == CWR_OK) rc = check_scores(R, V, tokens, M, K);
+    if (rc != CWR_OK) return rc;
+    if (H < 32 || H % 32 != 0) return CWR_ERR_SHAPE;
+    if (H > 0x3fffffff || R > 0x3fffffffLL * 4) return CWR_ERR_TOO_LARGE;
+    if (R > 0 && (!w || !workspace || (M > 0 && !logprobs) || (K > 0 && (!top_logprobs || !top_index))))
+        return CWR_ERR_NULL;
+    if (misaligned(h, 16) || misaligned(w, 16) || misaligned(bias, bias_dtype == CWR_F32 ? 4 : 2) ||
+        misaligned(workspace, 256) || misaligned(logprobs, 4) || misaligned(entropy, 4) || misaligned(lse, 4) ||
+        misaligned(top_logprobs, 4) || misaligned(top_index, 4) || misaligned(status, 4))
+        return CWR_ERR_ALIGN;
+    const RowScores s = {tokens, M, K, nullptr, logprobs, entropy, lse, top_logprobs, top_index, status};
+    return launch_joint_scores(h, w, bias, bias_dtype, dtype, R, H, V, temperature, s, workspace, workspace_bytes_,
+                               static_cast<hipStream_t>(stream));
 }
 
 size_t cwr_distill_workspace_bytes(void) { return sum_workspace_bytes(); }
@@ -635,16 +661,16 @@ static int check_distill(int64_t R, const float* top, const int32_t* top_index, 
 
 int cwr_distill(const void* x, int dtype, int64_t R, int64_t V, int64_t x_stride, const float* top,
                 const int32_t* top_index, int64_t K, double temperature, int tail, float* loss, float* stat,
-                float* reduced, void* workspace, int32_t* status, void* stream) {
+                float* loss_sum, float* loss_mean, void* workspace, int32_t* status, void* stream) {
     int rc = check_rows(x, dtype, R, V, x_stride, K, temperature);
     if (rc == CWR_OK) rc = check_distill(R, top, top_index, K, tail);
     if (rc != CWR_OK) return rc;
-    if ((R > 0 && !loss) || (reduced && !workspace)) return CWR_ERR_NULL;
-    if (misaligned(loss, 4) || misaligned(stat, 16) || misaligned(reduced, 4) || misaligned(workspace, 8) ||
-        misaligned(status, 4))
+    if ((R > 0 && !loss) || ((loss_sum || loss_mean) && !workspace)) return CWR_ERR_NULL;
+    if (misaligned(loss, 4) || misaligned(stat, 16) || misaligned(loss_sum, 4) || misaligned(loss_mean, 4) ||
+        misaligned(workspace, 8) || misaligned(status, 4))
         return CWR_ERR_ALIGN;
     const RowDistill s = {top, top_index, K, tail != 0, stat};
-    return launch_distill(x, dtype, R, V, x_stride, temperature, s, loss, reduced, workspace, status,
+    return launch_distill(x, dtype, R, V, x_stride, temperature, s, loss, loss_sum, loss_mean, workspace, status,
                           static_cast<hipStream_t>(stream));
 }
 

@@ -123,7 +123,6 @@ struct RowScores {
 };
 struct RowScoreGrads {
     const float* stat;
-    const float* entropy;
     const int* tokens;
     const int* top_index;
     i64 M, K;
@@ -137,6 +136,12 @@ int launch_scores(const void* x, int dtype, i64 R, i64 V, i64 stride, double tem
 int launch_scores_grad(const void* x, int dtype, i64 R, i64 V, i64 stride, double temperature, const RowScoreGrads& s,
                        void* dx, hipStream_t stream);
 
+// Scores of h (R,H) x W^T (V,H) + bias, the logits a block of rows at a time in the workspace (joint_scores.hip)
+size_t joint_scores_workspace_bytes(i64 R, i64 V);
+int launch_joint_scores(const void* h, const void* w, const void* bias, int bias_dtype, int dtype, i64 R, i64 H, i64 V,
+                        double temperature, const RowScores& s, void* workspace, size_t workspace_bytes,
+                        hipStream_t stream);
+
 // Distillation of rows of logits (distill.hip): pointers as in cwr_distill / cwr_distill_backward
 struct RowDistill {
     const float* top;
@@ -147,7 +152,7 @@ struct RowDistill {
 };
 size_t sum_workspace_bytes();
 int launch_distill(const void* x, int dtype, i64 R, i64 V, i64 stride, double temperature, const RowDistill& s,
-                   float* loss, float* reduced, void* workspace, int* status, hipStream_t stream);
+                   float* loss, float* loss_sum, float* loss_mean, void* workspace, int* status, hipStream_t stream);
 int launch_distill_grad(const void* x, int dtype, i64 R, i64 V, i64 stride, double temperature, const RowDistill& s,
                         const GradOut go, void* dx, hipStream_t stream);
 

@@ -232,21 +232,22 @@ __global__ __launch_bounds__(kSumThreads) void k_sum_rows(const float* __restric
 }
 
 template <typename S>
-__global__ __launch_bounds__(kSumThreads) void k_sum_mean(const S* __restrict__ v, i64 n, i64 R, float* __restrict__ out) {
+__global__ __launch_bounds__(kSumThreads) void k_sum_mean(const S* __restrict__ v, i64 n, i64 R, float* __restrict__ sum,
+                                                          float* __restrict__ mean) {
     double s = 0.0;
     for (i64 i = threadIdx.x; i < n; i += kSumThreads) s += (double)v[i];
     s = block_sum(s);
     if (threadIdx.x == 0) {
-        out[0] = (float)s;
-        out[1] = (float)(s / (double)R);
+        if (sum) *sum = (float)s;
+        if (mean) *mean = (float)(s / (double)R);
     }
 }
 
 size_t sum_workspace_bytes() { return kSumBlocks * sizeof(double); }
 
-static int launch_sum_mean(const float* rows, i64 R, double* work, float* out, hipStream_t stream) {
+static int launch_sum_mean(const float* rows, i64 R, double* work, float* sum, float* mean, hipStream_t stream) {
     if (R <= 16 * kSumThreads) {
-        CWR_LAUNCH((k_sum_mean<float>), dim3(1), dim3(kSumThreads), 0, stream, rows, R, R, out);
+        CWR_LAUNCH((k_sum_mean<float>), dim3(1), dim3(kSumThreads), 0, stream, rows, R, R, sum, mean);
         return check_launch();
     }
     const i64 want = (R + 4 * kSumThreads - 1) / (4 * kSumThreads);
@@ -254,7 +255,7 @@ static int launch_sum_mean(const float* rows, i64 R, double* work, float* out, h
     CWR_LAUNCH(k_sum_rows, dim3((unsigned)blocks), dim3(kSumThreads), 0, stream, rows, R, work);
     const int rc = check_launch();
     if (rc != CWR_OK) return rc;
-    CWR_LAUNCH((k_sum_mean<double>), dim3(1), dim3(kSumThreads), 0, stream, work, (i64)blocks, R, out);
+    CWR_LAUNCH((k_sum_mean<double>), dim3(1), dim3(kSumThreads), 0, stream, work, (i64)blocks, R, sum, mean);
     return check_launch();
 }
 
@@ -436,7 +437,7 @@ static int distill_grad_any(const void* x, i64 R, int V, i64 stride, const Tempe
 }
 
 int launch_distill(const void* x, int dtype, i64 R, i64 V, i64 stride, double temperature, const RowDistill& s,
-                   float* loss, float* reduced, void* workspace, int* status, hipStream_t stream) {
+                   float* loss, float* loss_sum, float* loss_mean, void* workspace, int* status, hipStream_t stream) {
     DistillArgs a;
     a.top = s.top; a.index = s.index; a.K = (int)s.K; a.loss = loss; a.stat = reinterpret_cast<float4*>(s.stat);
     a.status = status;
@@ -451,8 +452,8 @@ int launch_distill(const void* x, int dtype, i64 R, i64 V, i64 stride, double te
             default: return CWR_ERR_DTYPE;
         }
     }
-    if (rc != CWR_OK || !reduced) return rc;
-    return launch_sum_mean(loss, R, static_cast<double*>(workspace), reduced, stream);
+    if (rc != CWR_OK || (!loss_sum && !loss_mean)) return rc;
+    return launch_sum_mean(loss, R, static_cast<double*>(workspace), loss_sum, loss_mean, stream);
 }
 
 int launch_distill_grad(const void* x, int dtype, i64 R, i64 V, i64 stride, double temperature, const RowDistill& s,

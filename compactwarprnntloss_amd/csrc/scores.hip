@@ -19,7 +19,7 @@ namespace cwr {
 struct ScoreArgs {
     const int* tokens;  // (R, M)
     int M, K;
-    float2* stat;  // (R) maximum, log2 of the sum of 2^((x - max) c); may be null
+    float4* stat;  // (R) maximum, log2 of the sum of 2^((x - max) c), entropy, 0; may be null
     float* logprobs;
     float* entropy;
     float* lse;
@@ -47,11 +47,12 @@ __device__ __forceinline__ void write_tokens(const T* __restrict__ row, i64 r, i
 // maximum m, l2 = log2_sum, o the row's sums: what is known of the row as a whole
 __device__ __forceinline__ void write_row(i64 r, const Online& o, float l2, const Temper& tp, const ScoreArgs& a) {
     const bool empty = o.m == -INFINITY;  // nothing but -inf
-    if (a.stat) a.stat[r] = make_float2(o.m, l2);
     if (a.lse) a.lse[r] = empty ? (l2 != l2 ? l2 : -INFINITY)
                                 : (float)((double)o.m * tp.inv + (double)l2 * 0.6931471805599453);
     // H = -sum p ln p with log2 p = t - log2(s): the slip of ms is in both and cancels
-    if (a.entropy) a.entropy[r] = empty ? (l2 != l2 ? l2 : 0.f) : kLn2 * (log2_of_sum(o.s) - o.u / o.s);
+    const float h = empty ? (l2 != l2 ? l2 : 0.f) : kLn2 * (log2_of_sum(o.s) - o.u / o.s);
+    if (a.entropy) a.entropy[r] = h;
+    if (a.stat) a.stat[r] = make_float4(o.m, l2, h, 0.f);
 }
 
 // log2_sum with the empty row's answer
@@ -363,8 +364,7 @@ __global__ __launch_bounds__(64 * (NW > 1 ? NW : kWavesPerBlock)) void k_scores_
 // backward
 // ---------------------------------------------------------------------------------------------
 struct ScoreGrads {
-    const float2* stat;
-    const float* entropy;  // needed with g_entropy
+    const float4* stat;
     const int* tokens;
     const int* top_index;
     int M, K;
@@ -452,7 +452,7 @@ __global__ __launch_bounds__(kWavesPerBlock * 64) void k_scores_grad(const T* __
     }
     wsum = group_allreduce<G, OpSum>(wsum);
 
-    const float2 st = a.stat[r];
+    const float4 st = a.stat[r];
     const float m = st.x, l2 = st.y;
     const bool empty = m == -INFINITY && l2 == l2;  // NaN rows stay NaN
     const Anchor anc = anchor(m, tp.c);
@@ -465,7 +465,7 @@ __global__ __launch_bounds__(kWavesPerBlock * 64) void k_scores_grad(const T* __
     if (a.g_entropy) {
         const float gh = a.g_entropy[r];
         k1 = -gh * kLn2;
-        k0 -= gh * (a.entropy[r] - kLn2 * (l2 + slip));
+        k0 -= gh * (st.z - kLn2 * (l2 + slip));
     }
     k1 *= rs;
     k0 *= rs;
@@ -581,7 +581,7 @@ int launch_scores(const void* x, int dtype, i64 R, i64 V, i64 stride, double tem
                   hipStream_t stream) {
     if (R == 0) return CWR_OK;
     ScoreArgs a;
-    a.tokens = s.tokens; a.M = (int)s.M; a.K = (int)s.K; a.stat = reinterpret_cast<float2*>(s.stat);
+    a.tokens = s.tokens; a.M = (int)s.M; a.K = (int)s.K; a.stat = reinterpret_cast<float4*>(s.stat);
     a.logprobs = s.logprobs; a.entropy = s.entropy; a.lse = s.lse;
     a.top_logprobs = s.top_logprobs; a.top_index = s.top_index; a.status = s.status;
     const Temper tp = make_temper(temperature);
@@ -598,7 +598,7 @@ int launch_scores_grad(const void* x, int dtype, i64 R, i64 V, i64 stride, doubl
                        void* dx, hipStream_t stream) {
     if (R == 0) return CWR_OK;
     ScoreGrads a;
-    a.stat = reinterpret_cast<const float2*>(s.stat); a.entropy = s.entropy; a.tokens = s.tokens;
+    a.stat = reinterpret_cast<const float4*>(s.stat); a.tokens = s.tokens;
     a.top_index = s.top_index; a.M = (int)s.M; a.K = (int)s.K; a.g_logprobs = s.g_logprobs;
     a.g_entropy = s.g_entropy; a.g_lse = s.g_lse; a.g_top = s.g_top;
     const Temper tp = make_temper(temperature);

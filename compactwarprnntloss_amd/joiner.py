@@ -15,6 +15,7 @@ import torch
 from . import _lib
 from .loss import (RESIDENT_JOINT_SIZES, _DTYPES, _offsets, _raise_on_flags, _raise_on_status, _stream_ptr,
                    joint_forward, joint_forward_fg)
+from .scores import TokenScores, joint_token_logprobs, lattice_tokens, token_logprobs
 
 _ACTS = {None: 0, "none": 0, "tanh": 1, "relu": 2}
 _DW_SPLIT = 16  # parts the rows of a block are cut into for the weight-gradient product
@@ -302,3 +303,32 @@ class CompactJoiner(torch.nn.Module):
         (fused_joiner_loss)."""
         return fused_joiner_loss(self.enc(enc_out), self.pred(pred_out), self.out.weight, self.out.bias, lx, y, ly,
                                  blank, reduction, self.activation, total_rows=total_rows)
+
+    def _row_scores(self, h, tokens, top_k, entropy, temperature):
+        if h.dtype in (torch.float16, torch.bfloat16) and h.size(1) % 32 == 0:
+            with torch.no_grad():
+                return joint_token_logprobs(h, self.out.weight, self.out.bias, tokens, top_k=top_k, entropy=entropy,
+                                            temperature=temperature)
+        return token_logprobs(self.out(h), tokens, top_k=top_k, entropy=entropy, temperature=temperature)
+
+    @torch.no_grad()
+    def lattice_scores(self, enc_out, pred_out, lx, y, ly, blank: int = 0, top_k: int = 0, entropy: bool = False,
+                       temperature: float = 1.0, total_rows: Optional[int] = None) -> TokenScores:
+        """Scores of every lattice cell without its logits (fp16 / bf16 modules; others go through stored
+        logits): logprobs (R, 2) of the blank and the cell's label (0 where a cell has no label), and on
+        request the entropy and the top_k most probable entries, in the row order of forward().  A teacher's
+        top_logprobs and top_index are what distill_loss(..., tail=True) takes.  No gradient."""
+        if total_rows is None:
+            total_rows = int((lx.long() * (ly.long() + 1)).sum().item())
+        h = compact_join(self.enc(enc_out), self.pred(pred_out), lx, ly, self.activation, total_rows)
+        tokens = lattice_tokens(lx, y, ly, total_rows, self.out.weight.size(0), blank)
+        return self._row_scores(h, tokens, top_k, entropy, temperature)
+
+    @torch.no_grad()
+    def step_scores(self, enc_frame, pred_state, tokens: Optional[torch.Tensor] = None, top_k: int = 1,
+                    entropy: bool = False, temperature: float = 1.0) -> TokenScores:
+        """One step of a search: row b scores act(enc(enc_frame[b]) + pred(pred_state[b])), (B, enc_dim) and
+        (B, pred_dim), e.g. one row per hypothesis.  tokens (B,) or (B, M) int32 or None.  No gradient."""
+        z = self.enc(enc_frame) + self.pred(pred_state)
+        h = torch.tanh(z) if self.activation == "tanh" else torch.relu(z) if self.activation == "relu" else z
+        return self._row_scores(h, tokens, top_k, entropy, temperature)

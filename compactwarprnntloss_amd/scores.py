@@ -32,6 +32,25 @@ def _ptr(t: Optional[torch.Tensor]):
     return t.data_ptr() if t is not None else None
 
 
+# The raw handle of a device's current stream: what torch.cuda.current_stream(device).cuda_stream returns,
+# without building the Stream object in between (2 us, a tenth of a small call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _call(name: str, device: torch.device, *args):
+    """Runs entry point `name` with `args` and the current stream of `device`, on that device."""
+    fn = getattr(_lib.load(), name)
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc, name)
+
+
 def _check_rows(x: torch.Tensor, temperature: float):
     if not x.is_cuda:
         raise RuntimeError("x must be a CUDA tensor")
@@ -73,53 +92,51 @@ def _new_status(device) -> torch.Tensor:
     return torch.zeros(4, dtype=torch.int32, device=device)
 
 
+def _run_scores(x, tokens, top_k, want_entropy, temperature, status, keep):
+    """Binding of cwr_token_logprobs: (logprobs, entropy, lse, top_logprobs, top_index, stat)."""
+    R, V = x.shape
+    dev = x.device
+    M = tokens.size(1) if tokens is not None else 0
+    f32 = torch.float32
+    logprobs = torch.empty((R, M), dtype=f32, device=dev) if M else None
+    entropy = torch.empty(R, dtype=f32, device=dev) if want_entropy else None
+    lse = torch.empty(R, dtype=f32, device=dev)
+    top = index = None
+    if top_k:
+        top = torch.empty((R, top_k), dtype=f32, device=dev)
+        index = torch.empty((R, top_k), dtype=torch.int32, device=dev)
+    stat = torch.empty((R, 4), dtype=f32, device=dev) if keep else None
+    _call("cwr_token_logprobs", dev, x.data_ptr(), _DTYPES[x.dtype], R, V, x.stride(0), _ptr(tokens), M, top_k,
+          temperature, _ptr(stat), _ptr(logprobs), _ptr(entropy), lse.data_ptr(), _ptr(top), _ptr(index), _ptr(status))
+    return logprobs, entropy, lse, top, index, stat
+
+
 class _TokenScores(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, x, tokens, top_k, want_entropy, temperature, status):
-        lib = _lib.load()
-        R, V = x.shape
-        dev = x.device
-        M = tokens.size(1) if tokens is not None else 0
-        need = ctx.needs_input_grad[0]
-
-        def f32(*shape):
-            return torch.empty(shape, dtype=torch.float32, device=dev)
-        stat = f32(R, 2) if need else None
-        logprobs = f32(R, M) if M else None
-        entropy = f32(R) if want_entropy else None
-        lse = f32(R)
-        top = f32(R, top_k) if top_k else None
-        index = torch.empty((R, top_k), dtype=torch.int32, device=dev) if top_k else None
-        with torch.cuda.device(dev):
-            rc = lib.cwr_token_logprobs(x.data_ptr(), _DTYPES[x.dtype], R, V, x.stride(0), _ptr(tokens), M, top_k,
-                                        temperature, _ptr(stat), _ptr(logprobs), _ptr(entropy), lse.data_ptr(),
-                                        _ptr(top), _ptr(index), _ptr(status), _stream_ptr(dev))
-            _lib.check(rc, "cwr_token_logprobs")
+        logprobs, entropy, lse, top, index, stat = _run_scores(x, tokens, top_k, want_entropy, temperature, status, True)
         if index is not None:
             ctx.mark_non_differentiable(index)
         ctx.set_materialize_grads(False)
-        if need:
-            ctx.temperature = temperature
-            ctx.save_for_backward(x, tokens, index, entropy, stat)
+        ctx.temperature = temperature
+        ctx.save_for_backward(x, tokens, index, stat)
         return logprobs, entropy, lse, top, index
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx: Any, g_logprobs, g_entropy, g_lse, g_top, _g_index):
-        x, tokens, index, entropy, stat = ctx.saved_tensors
-        lib = _lib.load()
+        x, tokens, index, stat = ctx.saved_tensors
         R, V = x.shape
-        dev = x.device
-        grads = [g.to(torch.float32).contiguous() if g is not None else None for g in (g_logprobs, g_entropy, g_lse, g_top)]
-        dx = torch.empty((R, V), dtype=x.dtype, device=dev)
-        with torch.cuda.device(dev):
-            rc = lib.cwr_token_logprobs_backward(
-                x.data_ptr(), _DTYPES[x.dtype], R, V, x.stride(0), _ptr(tokens),
-                tokens.size(1) if tokens is not None else 0, _ptr(index), index.size(1) if index is not None else 0,
-                ctx.temperature, stat.data_ptr(), _ptr(entropy), *[_ptr(g) for g in grads], dx.data_ptr(),
-                _stream_ptr(dev))
-            _lib.check(rc, "cwr_token_logprobs_backward")
+        grads = [g if g is None else _rows_f32(g) for g in (g_logprobs, g_entropy, g_lse, g_top)]
+        dx = torch.empty((R, V), dtype=x.dtype, device=x.device)
+        _call("cwr_token_logprobs_backward", x.device, x.data_ptr(), _DTYPES[x.dtype], R, V, x.stride(0), _ptr(tokens),
+              tokens.size(1) if tokens is not None else 0, _ptr(index), index.size(1) if index is not None else 0,
+              ctx.temperature, stat.data_ptr(), *[_ptr(g) for g in grads], dx.data_ptr())
         return dx, None, None, None, None, None
+
+
+def _rows_f32(g: torch.Tensor) -> torch.Tensor:
+    return g if g.dtype == torch.float32 and g.is_contiguous() else g.to(torch.float32).contiguous()
 
 
 def token_logprobs(x: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, top_k: int = 0, entropy: bool = False,
@@ -143,8 +160,11 @@ def token_logprobs(x: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, to
     R, V = x.shape
     rows = _check_tokens(tokens, R, x.device)
     status = _new_status(x.device) if validate else None
-    logprobs, ent, lse, top, index = _TokenScores.apply(x, rows, _check_top_k(top_k, V), bool(entropy), temperature,
-                                                        status)
+    top_k = _check_top_k(top_k, V)
+    if x.requires_grad and torch.is_grad_enabled():
+        logprobs, ent, lse, top, index = _TokenScores.apply(x, rows, top_k, bool(entropy), temperature, status)
+    else:
+        logprobs, ent, lse, top, index, _ = _run_scores(x, rows, top_k, bool(entropy), temperature, status, False)
     if validate:
         _raise_on_status(status, "token_logprobs")
     if tokens is not None and tokens.dim() == 1:
@@ -152,47 +172,102 @@ def token_logprobs(x: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, to
     return TokenScores(logprobs, ent, lse, top, index)
 
 
+def joint_token_logprobs(h: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                         tokens: Optional[torch.Tensor] = None, *, top_k: int = 0, entropy: bool = False,
+                         temperature: float = 1.0, validate: bool = False) -> TokenScores:
+    """token_logprobs of the logits h @ weight.T + bias without storing them: h (R, H) joint rows (from
+    compact_join, or one row per hypothesis of a search), weight (V, H), both fp16 or both bf16 with H a
+    multiple of 32; bias (V,) in the same type or fp32, or None.  The product runs on the matrix cores with
+    fp32 accumulation and is scored from fp32, a block of rows at a time (at most 128 MiB, or 4096 rows).
+
+    For a teacher's pass over a lattice and for the steps of a search: the scores carry no gradient, and a
+    call that would need one is refused."""
+    temperature = float(temperature)
+    _check_rows(h, temperature)
+    if h.dtype not in (torch.float16, torch.bfloat16) or weight.dtype != h.dtype:
+        raise RuntimeError("h and weight must both be float16 or both be bfloat16")
+    if weight.dim() != 2 or weight.size(1) != h.size(1) or weight.size(0) < 1:
+        raise RuntimeError("weight must be (V, H) with the joint dimension H of the rows")
+    if h.size(1) % 32 != 0:
+        raise RuntimeError("the joint dimension must be a multiple of 32")
+    dev = h.device
+    if weight.device != dev or (bias is not None and bias.device != dev):
+        raise RuntimeError("weight and bias must be on the device of h")
+    if not h.is_contiguous() or not weight.is_contiguous():
+        raise RuntimeError("h and weight must be contiguous")
+    R, H = h.shape
+    V = weight.size(0)
+    if bias is not None and (bias.shape != (V,) or bias.dtype not in (h.dtype, torch.float32) or not bias.is_contiguous()):
+        raise RuntimeError("bias must hold one value per vocabulary entry, in the type of h or fp32")
+    if torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        raise RuntimeError("joint_token_logprobs has no gradient: call it under torch.no_grad(), or use "
+                           "token_logprobs on stored logits")
+    rows = _check_tokens(tokens, R, dev)
+    top_k = _check_top_k(top_k, V)
+    status = _new_status(dev) if validate else None
+    M = rows.size(1) if rows is not None else 0
+    f32 = torch.float32
+    logprobs = torch.empty((R, M), dtype=f32, device=dev) if M else None
+    ent = torch.empty(R, dtype=f32, device=dev) if entropy else None
+    lse = torch.empty(R, dtype=f32, device=dev)
+    top = index = None
+    if top_k:
+        top = torch.empty((R, top_k), dtype=f32, device=dev)
+        index = torch.empty((R, top_k), dtype=torch.int32, device=dev)
+    nbytes = _lib.load().cwr_joint_token_logprobs_workspace_bytes(R, V)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _call("cwr_joint_token_logprobs", dev, h.data_ptr(), weight.data_ptr(), _ptr(bias),
+          _DTYPES[bias.dtype] if bias is not None else _lib.F32, _DTYPES[h.dtype], R, H, V, _ptr(rows), M, top_k,
+          temperature, _ptr(logprobs), _ptr(ent), lse.data_ptr(), _ptr(top), _ptr(index), work.data_ptr(), nbytes,
+          _ptr(status))
+    if validate:
+        _raise_on_status(status, "joint_token_logprobs")
+    if tokens is not None and tokens.dim() == 1:
+        logprobs = logprobs.view(R)
+    return TokenScores(logprobs, ent, lse, top, index)
+
+
+def _run_distill(x, top, index, temperature, tail, reduction, status, keep):
+    """Binding of cwr_distill: (loss, stat)."""
+    R, V = x.shape
+    dev = x.device
+    # what the backward pass needs and, under a reduction, its workspace and the rows' losses
+    work_floats = _lib.load().cwr_distill_workspace_bytes() // 4
+    buf = torch.empty(4 * R + (work_floats + R if reduction != "none" else 0), dtype=torch.float32, device=dev)
+    base = buf.data_ptr()
+    total = mean = work = None
+    if reduction == "none":
+        loss = torch.empty(R, dtype=torch.float32, device=dev)
+        rows = loss.data_ptr()
+    else:
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        work, rows = base + 16 * R, base + 16 * R + 4 * work_floats
+        total, mean = (loss.data_ptr(), None) if reduction == "sum" else (None, loss.data_ptr())
+    _call("cwr_distill", dev, x.data_ptr(), _DTYPES[x.dtype], R, V, x.stride(0), top.data_ptr(), index.data_ptr(),
+          index.size(1), temperature, int(tail), rows, base if keep else None, total, mean, work, _ptr(status))
+    return loss, buf
+
+
 class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, x, top, index, temperature, tail, reduction, status):
-        lib = _lib.load()
-        R, V = x.shape
-        dev = x.device
-        need = ctx.needs_input_grad[0]
-        loss = torch.empty(R, dtype=torch.float32, device=dev)
-        stat = torch.empty((R, 4), dtype=torch.float32, device=dev) if need else None
-        reduced = work = None
-        if reduction != "none":
-            reduced = torch.empty(2, dtype=torch.float32, device=dev)
-            work = torch.empty(lib.cwr_distill_workspace_bytes(), dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev):
-            rc = lib.cwr_distill(x.data_ptr(), _DTYPES[x.dtype], R, V, x.stride(0), top.data_ptr(), index.data_ptr(),
-                                 index.size(1), temperature, int(tail), loss.data_ptr(), _ptr(stat), _ptr(reduced),
-                                 _ptr(work), _ptr(status), _stream_ptr(dev))
-            _lib.check(rc, "cwr_distill")
-        if need:
-            ctx.temperature, ctx.tail, ctx.reduction = temperature, tail, reduction
-            ctx.save_for_backward(x, top, index, stat)
-        if reduction == "none":
-            return loss
-        return reduced[1 if reduction == "mean" else 0]
+        loss, stat = _run_distill(x, top, index, temperature, tail, reduction, status, True)
+        ctx.temperature, ctx.tail, ctx.reduction = temperature, tail, reduction
+        ctx.save_for_backward(x, top, index, stat)
+        return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx: Any, grad_out):
         x, top, index, stat = ctx.saved_tensors
-        lib = _lib.load()
         R, V = x.shape
-        dev = x.device
-        go = grad_out.to(torch.float32).contiguous()
+        go = _rows_f32(grad_out)
         stride = 1 if ctx.reduction == "none" else 0
         scale = 1.0 / R if ctx.reduction == "mean" and R else 1.0
-        dx = torch.empty((R, V), dtype=x.dtype, device=dev)
-        with torch.cuda.device(dev):
-            rc = lib.cwr_distill_backward(x.data_ptr(), _DTYPES[x.dtype], R, V, x.stride(0), top.data_ptr(),
-                                          index.data_ptr(), index.size(1), ctx.temperature, int(ctx.tail),
-                                          stat.data_ptr(), go.data_ptr(), stride, scale, dx.data_ptr(), _stream_ptr(dev))
-            _lib.check(rc, "cwr_distill_backward")
+        dx = torch.empty((R, V), dtype=x.dtype, device=x.device)
+        _call("cwr_distill_backward", x.device, x.data_ptr(), _DTYPES[x.dtype], R, V, x.stride(0), top.data_ptr(),
+              index.data_ptr(), index.size(1), ctx.temperature, int(ctx.tail), stat.data_ptr(), go.data_ptr(), stride,
+              scale, dx.data_ptr())
         return dx, None, None, None, None, None, None
 
 
@@ -230,8 +305,12 @@ def distill_loss(x: torch.Tensor, top_logits: torch.Tensor, top_index: torch.Ten
     if torch.is_grad_enabled() and top_logits.requires_grad:
         raise RuntimeError("the teacher gets no gradient: pass top_logits.detach()")
     status = _new_status(x.device) if validate else None
-    loss = _Distill.apply(x, top_logits.to(torch.float32).contiguous(), top_index.contiguous(), temperature, bool(tail),
-                          reduction if reduction in ("mean", "sum") else "none", status)
+    reduction = reduction or "none"
+    top = _rows_f32(top_logits.detach())
+    if x.requires_grad and torch.is_grad_enabled():
+        loss = _Distill.apply(x, top, top_index.contiguous(), temperature, bool(tail), reduction, status)
+    else:
+        loss, _ = _run_distill(x, top, top_index.contiguous(), temperature, bool(tail), reduction, status, False)
     if validate:
         _raise_on_status(status, "distill_loss")
     return loss

@@ -347,7 +347,8 @@ int cwr_joint_backward(const void* h, const void* w, const float* bias, int dtyp
  *   x            (R, V) of any cwr_dtype (64-bit entries are rounded to fp32 when read, as everywhere in
  *                this library), row r at x + r * x_stride, entries of a row adjacent; x_stride >= 0
  *   tokens       (R, M) int32, M <= 64;  K <= 64, K <= V;  temperature > 0 and finite
- *   stat         (R, 2) fp32 for cwr_token_logprobs_backward: row maximum, log2 of the scaled sum;  NULL: not kept
+ *   stat         (R, 4) fp32, 16-byte aligned, for cwr_token_logprobs_backward: row maximum, log2 of the scaled
+ *                sum, entropy, 0;  NULL: not kept
  *   logprobs     (R, M) fp32, NULL only if M = 0;  entropy, lse (R) fp32, each may be NULL
  *   top_logprobs (R, K) fp32 and top_index (R, K) int32, NULL only if K = 0
  *   status       4 x int32 the caller has zeroed, or NULL
@@ -360,12 +361,27 @@ int cwr_token_logprobs(const void* x, int dtype, int64_t R, int64_t V, int64_t x
 
 /* Backward of cwr_token_logprobs: dx (R, V) of `dtype`, contiguous, every element written.  g_logprobs
  * (R, M), g_entropy (R), g_lse (R), g_top (R, K) fp32 are the gradients of its outputs, each may be NULL
- * (zero); tokens of -1 or outside [0, V) get none.  stat, entropy (needed with g_entropy) and top_index
- * as that call wrote them; all other arguments as there. */
+ * (zero); tokens of -1 or outside [0, V) get none.  stat and top_index as that call wrote them; all other
+ * arguments as there. */
 int cwr_token_logprobs_backward(const void* x, int dtype, int64_t R, int64_t V, int64_t x_stride,
                                 const int32_t* tokens, int64_t M, const int32_t* top_index, int64_t K,
-                                double temperature, const float* stat, const float* entropy, const float* g_logprobs,
-                                const float* g_entropy, const float* g_lse, const float* g_top, void* dx, void* stream);
+                                double temperature, const float* stat, const float* g_logprobs, const float* g_entropy,
+                                const float* g_lse, const float* g_top, void* dx, void* stream);
+
+/* cwr_token_logprobs of logits that are never stored as a whole: x[r, v] = sum_k h[r, k] * w[v, k] + bias[v]
+ * is formed on the matrix cores (16-bit inputs, fp32 accumulation) a block of rows at a time, in fp32, in
+ * the workspace, and scored there.  For a teacher's pass over the rows of a lattice and, with few
+ * rows, for a step of a search.  No gradient.
+ *   h     (R, H), w (V, H) of `dtype` = CWR_F16 or CWR_BF16, contiguous, 16-byte aligned; H a multiple of 32
+ *   bias  (V,) of `bias_dtype` = CWR_F32 or `dtype`, or NULL
+ *   workspace  256-byte aligned; cwr_joint_token_logprobs_workspace_bytes(R, V) bytes are enough to run
+ *         well, less (down to one row, V rounded up to a multiple of 4, of fp32) means more, smaller blocks
+ * All other arguments and outputs as for cwr_token_logprobs. */
+size_t cwr_joint_token_logprobs_workspace_bytes(int64_t R, int64_t V);
+int cwr_joint_token_logprobs(const void* h, const void* w, const void* bias, int bias_dtype, int dtype, int64_t R,
+                             int64_t H, int64_t V, const int32_t* tokens, int64_t M, int64_t K, double temperature,
+                             float* logprobs, float* entropy, float* lse, float* top_logprobs, int32_t* top_index,
+                             void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
 
 /* Distillation of rows of logits from a teacher's top logits.  z = x[r, :] / temperature, p = softmax(z);
  * the teacher's entry k of row r is index top_index[r, k] with value top[r, k]; an index of -1 is absent.
@@ -382,12 +398,12 @@ int cwr_token_logprobs_backward(const void* x, int dtype, int64_t R, int64_t V, 
  *   x, dtype, x_stride, temperature, status as for cwr_token_logprobs
  *   top (R, K) fp32, top_index (R, K) int32, 1 <= K <= 64
  *   loss (R) fp32;  stat (R, 4) fp32, 16-byte aligned, for cwr_distill_backward, NULL: not kept
- *   reduced      NULL, or 2 x fp32: sum and mean of the losses, added in 64 bits in a fixed order; needs
- *                workspace of cwr_distill_workspace_bytes() bytes, 8-byte aligned (else NULL) */
+ *   loss_sum, loss_mean  1 x fp32 each or NULL: sum and mean of the losses, added in 64 bits in a fixed
+ *                order; either needs workspace of cwr_distill_workspace_bytes() bytes, 8-byte aligned */
 size_t cwr_distill_workspace_bytes(void);
 int cwr_distill(const void* x, int dtype, int64_t R, int64_t V, int64_t x_stride, const float* top,
                 const int32_t* top_index, int64_t K, double temperature, int tail, float* loss, float* stat,
-                float* reduced, void* workspace, int32_t* status, void* stream);
+                float* loss_sum, float* loss_mean, void* workspace, int32_t* status, void* stream);
 
 /* Backward of cwr_distill: dx (R, V) of `dtype`, contiguous, every element written.
  *   dx[r, v] = g T (p[v] Q - sum_{k: i_k = v} q_k - [v not listed] q_r p[v] / p_r),   Q = sum q (+ q_r),
