@@ -145,17 +145,13 @@ template <int N> __device__ __forceinline__ void subtract_far(float (&v)[N], con
     }
 }
 
-template <bool ENTROPY>
-__device__ __forceinline__ void online_chunk(const float (&x)[kLaneElems], float m, float c, float& s, float& u) {
-    const Anchor a = anchor(m, c);
-    float v[kLaneElems];
-#pragma unroll
-    for (int i = 0; i < kLaneElems; ++i) v[i] = x[i];
-    subtract_far(v, a);
+template <bool ENTROPY, bool FAR>
+__device__ __forceinline__ void online_chunk_as(const float (&v)[kLaneElems], const Anchor& a, float c, float& s, float& u) {
     float sa = 0.f, sb = 0.f, ua = 0.f, ub = 0.f;
 #pragma unroll
     for (int i = 0; i < kLaneElems; i += 2) {
-        const float t0 = fmaf(v[i], c, -a.ms), t1 = fmaf(v[i + 1], c, -a.ms);
+        const float t0 = FAR ? measure(v[i], a, c) : fmaf(v[i], c, -a.ms);
+        const float t1 = FAR ? measure(v[i + 1], a, c) : fmaf(v[i + 1], c, -a.ms);
         const float e0 = fast_exp2(t0), e1 = fast_exp2(t1);
         sa += e0;
         sb += e1;
@@ -166,6 +162,12 @@ __device__ __forceinline__ void online_chunk(const float (&x)[kLaneElems], float
     }
     s = sa + sb;
     u = ua + ub;
+}
+template <bool ENTROPY>
+__device__ __forceinline__ void online_chunk(const float (&v)[kLaneElems], float m, float c, float& s, float& u) {
+    const Anchor a = anchor(m, c);
+    if (__ballot(a.sub != 0.f) != 0) online_chunk_as<ENTROPY, true>(v, a, c, s, u);
+    else online_chunk_as<ENTROPY, false>(v, a, c, s, u);
 }
 
 // state o measured against a maximum mn at least as large
@@ -179,11 +181,17 @@ __device__ __forceinline__ void online_rebase(Online& o, float mn, float c) {
     }
 }
 
+// Largest of a lane's values, NaN left out where there is a number.  As three-way maxima written out: around
+// fmaxf of values just loaded the compiler puts one more instruction per value, to quiet signalling NaNs.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 __device__ __forceinline__ float chunk_max(const float (&v)[kLaneElems]) {
-    float m = v[0];
-#pragma unroll
-    for (int i = 1; i < kLaneElems; ++i) m = fmaxf(m, v[i]);
-    return m;
+    const float a = max3(v[0], v[1], v[2]), b = max3(v[3], v[4], v[5]), c = max3(v[6], v[7], v[8]);
+    const float d = max3(v[9], v[10], v[11]), e = max3(v[12], v[13], v[14]);
+    return max3(max3(a, b, c), max3(d, e, v[15]), v[15]);
 }
 
 // log2 of the sum of 2^((x - m) c) from the sum s of 2^(x c - ms)

@@ -210,7 +210,7 @@ __global__ __launch_bounds__(64 * (NW > 1 ? NW : kWavesPerBlock)) void k_distill
 // ---------------------------------------------------------------------------------------------
 // sum and mean of the rows' losses, in a fixed order, in 64 bits
 // ---------------------------------------------------------------------------------------------
-constexpr int kSumBlocks = 256;
+constexpr int kSumBlocks = 1024;
 constexpr int kSumThreads = 256;
 
 __device__ __forceinline__ double block_sum(double v) {
@@ -226,7 +226,14 @@ __device__ __forceinline__ double block_sum(double v) {
 
 __global__ __launch_bounds__(kSumThreads) void k_sum_rows(const float* __restrict__ v, i64 n, double* __restrict__ part) {
     double s = 0.0;
-    for (i64 i = (i64)blockIdx.x * kSumThreads + threadIdx.x; i < n; i += (i64)gridDim.x * kSumThreads) s += (double)v[i];
+    const i64 step = (i64)gridDim.x * kSumThreads;
+    for (i64 i = (i64)blockIdx.x * kSumThreads + threadIdx.x; i < n; i += 4 * step) {  // four loads in flight
+        float f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = i + j * step < n ? v[i + j * step] : 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s += (double)f[j];
+    }
     s = block_sum(s);
     if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
@@ -353,7 +360,7 @@ __global__ __launch_bounds__(kWavesPerBlock * 64) void k_distill_grad(
         }
         if (!ok || el >= V) continue;
         if (!EDGE || (el >= 0 && el + VEC <= V)) {
-            store_raw<true>(out + el, Pack<T>::pack(d));
+            store_raw<G == 64 || (!EDGE && G >= 8)>(out + el, Pack<T>::pack(d));
         } else {
 #pragma unroll
             for (int j = 0; j < VEC; ++j)

@@ -28,20 +28,31 @@ struct ScoreArgs {
     int* status;  // may be null
 };
 
-// The row's scores of the given tokens, written by the G lanes that share the row (l: lane in group).
-template <typename T, int G>
-__device__ __forceinline__ void write_tokens(const T* __restrict__ row, i64 r, int l, int V, float m, float l2,
-                                             const Temper& tp, const ScoreArgs& a) {
-    for (int j = l; j < a.M; j += G) {
-        const int tok = a.tokens[r * a.M + j];
-        float lp = 0.f;  // -1: no token
-        if (tok >= 0 && tok < V) lp = logprob(Elem<T>::to_f32(row[tok]), m, l2, tp);
-        else if (tok != -1) {
-            lp = __int_as_float(0x7fc00000);
-            if (a.status) raise_flag(a.status, CWR_FLAG_BAD_LABEL);
-        }
-        a.logprobs[r * a.M + j] = lp;
+// The given tokens of a row, one per lane of the G lanes that share it (and round), in two steps: their
+// logits are asked for along with the row itself, so that nothing waits for them at the end.
+struct TokenLogit {
+    int tok;
+    float x;
+};
+template <typename T>
+__device__ __forceinline__ TokenLogit fetch_token(const T* __restrict__ row, i64 r, int j, int V, const ScoreArgs& a) {
+    TokenLogit t = {-1, 0.f};
+    if (j < a.M) {
+        t.tok = a.tokens[r * a.M + j];
+        if ((unsigned)t.tok < (unsigned)V) t.x = Elem<T>::to_f32(row[t.tok]);
     }
+    return t;
+}
+__device__ __forceinline__ void write_token(const TokenLogit& t, i64 r, int j, int V, float m, float l2, const Temper& tp,
+                                            const ScoreArgs& a) {
+    if (j >= a.M) return;
+    float lp = 0.f;  // -1: no token
+    if ((unsigned)t.tok < (unsigned)V) lp = logprob(t.x, m, l2, tp);
+    else if (t.tok != -1) {
+        lp = __int_as_float(0x7fc00000);
+        if (a.status) raise_flag(a.status, CWR_FLAG_BAD_LABEL);
+    }
+    a.logprobs[r * a.M + j] = lp;
 }
 
 // maximum m, l2 = log2_sum, o the row's sums: what is known of the row as a whole
@@ -89,6 +100,7 @@ __global__ __launch_bounds__(kWavesPerBlock * 64) void k_scores_group(const T* _
     v4i raw[NP];
 #pragma unroll
     for (int i = 0; i < NP; ++i) raw[i] = load_pack<T, EDGE, true>(row, (i * G + l) * VEC - off, V);
+    const TokenLogit tok = fetch_token<T>(row, ok ? r : R - 1, l, V, a);
     float v[kLaneElems];
     unpack_chunk<T>(raw, v);
     Online o;
@@ -98,7 +110,10 @@ __global__ __launch_bounds__(kWavesPerBlock * 64) void k_scores_group(const T* _
     o.u = group_allreduce<G, OpSum>(o.u);
     const float l2 = row_l2(o, tp.c);
     if (ok && l == 0) write_row(r, o, l2, tp, a);
-    if (ok && a.M > 0) write_tokens<T, G>(row, r, l, V, o.m, l2, tp, a);
+    if (ok) {
+        write_token(tok, r, l, V, o.m, l2, tp, a);
+        for (int j = l + G; j < a.M; j += G) write_token(fetch_token<T>(row, r, j, V, a), r, j, V, o.m, l2, tp, a);
+    }
     if (a.K == 0) return;
     int key[kLaneElems];
 #pragma unroll
@@ -147,7 +162,7 @@ __global__ __launch_bounds__(kWavesPerBlock * 64) void k_scores_group(const T* _
 // are at least their K-th largest, so K entries of the row are, and in rows of random order few more
 // (16 values a lane: 9 candidates on average for K = 8).  That costs 16 compares and about ten ballots a
 // row where one round of striking out (above) costs a hundred instructions per alternative.
-constexpr int kListCap = 256;
+constexpr int kListCap = 128;
 
 __device__ __forceinline__ u64 key_of(float f, int e) {
     const unsigned o = (unsigned)order_i32(f) ^ 0x80000000u;
@@ -159,28 +174,26 @@ __device__ __forceinline__ int key_index(u64 k) { return (int)(0xffffffffu - (un
 // The best min(n, K) of the n keys of a wave's list, sorted, in its first places.  Returns how many.
 __device__ __forceinline__ int list_compress(u64* list, int n, int K) {
     const int lane = threadIdx.x & 63;
-    u64 mine[kListCap / 64];
-    int rank[kListCap / 64];
-#pragma unroll
-    for (int s = 0; s < kListCap / 64; ++s) {
-        mine[s] = lane + 64 * s < n ? list[lane + 64 * s] : 0;
-        rank[s] = 0;
-    }
+    const u64 a = lane < n ? list[lane] : 0;
+    int ra = 0;
     if (n <= 64) {
-#pragma unroll 4
-        for (int c = 0; c < n; ++c) rank[0] += list[c] > mine[0] ? 1 : 0;
+#pragma unroll 2
+        for (int c = 0; c < n; ++c) ra += list[c] > a ? 1 : 0;
+        wave_sync();
+        if (lane < n && ra < K) list[ra] = a;
     } else {
-#pragma unroll 4
+        const u64 b = lane + 64 < n ? list[lane + 64] : 0;
+        int rb = 0;
+#pragma unroll 2
         for (int c = 0; c < n; ++c) {
             const u64 other = list[c];
-#pragma unroll
-            for (int s = 0; s < kListCap / 64; ++s) rank[s] += other > mine[s] ? 1 : 0;
+            ra += other > a ? 1 : 0;
+            rb += other > b ? 1 : 0;
         }
+        wave_sync();
+        if (ra < K) list[ra] = a;
+        if (lane + 64 < n && rb < K) list[rb] = b;
     }
-    wave_sync();
-#pragma unroll
-    for (int s = 0; s < kListCap / 64; ++s)
-        if (lane + 64 * s < n && rank[s] < K) list[rank[s]] = mine[s];
     wave_sync();
     return n < K ? n : K;
 }
@@ -222,45 +235,37 @@ __device__ __forceinline__ void rank_append(Ranking& q, float f, int e, bool in)
 }
 
 template <int VEC>
-__device__ __forceinline__ void rank_chunk(Ranking& q, const float (&v)[kLaneElems], int e0, int V, int K) {
-    u64 reach[kLaneElems];
-    int total = q.n;
+__device__ __forceinline__ void rank_chunk(Ranking& q, const float (&v)[kLaneElems], float best, int e0, int V, int K) {
+    if (__ballot(best >= q.floor_) == 0) return;
+    // every lane notes which of its values reach the bound; all lanes then hand in one of them at a time
+    // (about one lane in eight has any, hardly one has two)
+    unsigned reach = 0;
 #pragma unroll
-    for (int s = 0; s < kLaneElems; ++s) {
-        reach[s] = __ballot(v[s] >= q.floor_);
-        total += __popcll(reach[s]);
-    }
-    if (total <= kListCap) {
-#pragma unroll
-        for (int s = 0; s < kLaneElems; ++s) {
-            if (reach[s] == 0) continue;
-            const int e = e0 + (s / VEC) * 64 * VEC + (s & (VEC - 1));
-            rank_append(q, v[s], e, v[s] >= q.floor_ && (unsigned)e < (unsigned)V);
-        }
-        wave_sync();
-        return;
-    }
-    // many equal or many rising values: the list is cut back, and the bound raised, as often as it fills up
-#pragma unroll 1
-    for (int s = 0; s < kLaneElems; ++s) {
-        float f = v[0];
-#pragma unroll
-        for (int i = 1; i < kLaneElems; ++i) f = i == s ? v[i] : f;
-        if (q.n + 64 > kListCap) {
+    for (int s = 0; s < kLaneElems; ++s) reach |= v[s] >= q.floor_ ? 1u << s : 0u;
+    for (;;) {
+        const u64 some = __ballot(reach != 0);
+        if (some == 0) break;
+        // many equal or many rising values: the list is cut back, and the bound raised, as often as it fills up
+        if (q.n + __popcll(some) > kListCap) {
             q.n = list_compress(q.list, q.n, K);
             if (q.n == K) {
                 q.bound = q.list[K - 1];
                 q.floor_ = key_value(q.bound);
             }
         }
+        const int s = __ffs((int)reach) - 1;  // -1: none left
+        float f = v[0];
+#pragma unroll
+        for (int i = 1; i < kLaneElems; ++i) f = i == s ? v[i] : f;
         const int e = e0 + (s / VEC) * 64 * VEC + (s & (VEC - 1));
-        rank_append(q, f, e, f >= q.floor_ && (unsigned)e < (unsigned)V);
+        rank_append(q, f, e, reach != 0 && (unsigned)e < (unsigned)V);
+        reach &= reach - 1;
         wave_sync();
     }
 }
 
 template <typename T, int NW, bool EDGE>
-__global__ __launch_bounds__(64 * (NW > 1 ? NW : kWavesPerBlock)) void k_scores_wave(
+__global__ __launch_bounds__(64 * (NW > 1 ? NW : kWavesPerBlock), sizeof(T) == 2 ? 8 : sizeof(T) == 4 ? 6 : 4) void k_scores_wave(
     const T* __restrict__ x, i64 R, int V, i64 stride, const Temper tp, const ScoreArgs a) {
     constexpr int VEC = RowPacks<T>::VEC, NP = RowPacks<T>::NP;
     constexpr int WB = NW > 1 ? NW : kWavesPerBlock;
@@ -285,11 +290,12 @@ __global__ __launch_bounds__(64 * (NW > 1 ? NW : kWavesPerBlock)) void k_scores_
             next[i] = load_pack<T, EDGE, true>(row, ch * CHUNK + (i * 64 + lane) * VEC - off, V);
     };
     if (first < chunks) fetch(first);
+    const TokenLogit tok = fetch_token<T>(row, r, lane, V, a);
     for (int ch = first; ch < chunks; ch += NW) {
         float v[kLaneElems];
         unpack_chunk<T>(next, v);
         if (ch + NW < chunks) fetch(ch + NW);
-        const float best = chunk_max(v);
+        float best = chunk_max(v);
         const float top = group_allreduce<64, OpMax>(best);
         online_rebase(o, fmaxf(o.m, top), tp.c);
         float s, u;
@@ -300,13 +306,14 @@ __global__ __launch_bounds__(64 * (NW > 1 ? NW : kWavesPerBlock)) void k_scores_
         if (__ballot(s != s) != 0) {  // NaN (or +inf) in the chunk: NaN ranks as -inf
 #pragma unroll
             for (int i = 0; i < kLaneElems; ++i) v[i] = fmaxf(v[i], -INFINITY);
+            best = fmaxf(best, -INFINITY);
         }
         if (ch == first) {
-            const int lo = kth_bound(order_i32(fmaxf(best, -INFINITY)), a.K);
+            const int lo = kth_bound(order_i32(best), a.K);
             q.floor_ = from_order_i32(lo);
             q.bound = (u64)((unsigned)lo ^ 0x80000000u) << 32;  // below every key of that value
         }
-        rank_chunk<VEC>(q, v, ch * CHUNK + lane * VEC - off, V, a.K);
+        rank_chunk<VEC>(q, v, best, ch * CHUNK + lane * VEC - off, V, a.K);
     }
 
     // the lanes' sums, then the waves'
@@ -330,20 +337,20 @@ __global__ __launch_bounds__(64 * (NW > 1 ? NW : kWavesPerBlock)) void k_scores_
                 o.u += p.u;
             }
         }
-        // four lists into one, until one is left
+        // two lists into one, until one is left
         if (a.K > 0) {
 #pragma unroll
-            for (int left = NW / 4; left >= 1; left /= 4) {
-                u64 mine[4];
+            for (int left = NW / 2; left >= 1; left /= 2) {
+                u64 mine[2];
 #pragma unroll
-                for (int s = 0; s < 4; ++s) mine[s] = w < left && lane < a.K ? lists[4 * w + s][lane] : 0;
+                for (int s = 0; s < 2; ++s) mine[s] = w < left && lane < a.K ? lists[2 * w + s][lane] : 0;
                 __syncthreads();
                 if (w < left) {
 #pragma unroll
-                    for (int s = 0; s < 4; ++s)
+                    for (int s = 0; s < 2; ++s)
                         if (lane < a.K) q.list[s * a.K + lane] = mine[s];
                     wave_sync();
-                    list_compress(q.list, 4 * a.K, a.K);
+                    list_compress(q.list, 2 * a.K, a.K);
                 }
                 __syncthreads();
             }
@@ -352,7 +359,7 @@ __global__ __launch_bounds__(64 * (NW > 1 ? NW : kWavesPerBlock)) void k_scores_
     }
     const float l2 = row_l2(o, tp.c);
     if (lane == 0) write_row(r, o, l2, tp, a);
-    if (a.M > 0) write_tokens<T, 64>(row, r, lane, V, o.m, l2, tp, a);
+    write_token(tok, r, lane, V, o.m, l2, tp, a);
     if (lane < a.K) {
         const u64 key = q.list[lane];
         a.top_index[r * a.K + lane] = key_index(key);
@@ -499,7 +506,7 @@ __global__ __launch_bounds__(kWavesPerBlock * 64) void k_scores_grad(const T* __
         }
         if (!ok || e >= V) continue;
         if (!EDGE || (e >= 0 && e + VEC <= V)) {
-            store_raw<true>(out + e, Pack<T>::pack(d));
+            store_raw<G == 64 || (!EDGE && G >= 8)>(out + e, Pack<T>::pack(d));
         } else {
 #pragma unroll
             for (int j = 0; j < VEC; ++j)
