@@ -580,7 +580,7 @@ int cwr_join_backward(const void* dh, const void* h, int dtype, int act, int64_t
 static int check_rows(const void* x, int dtype, int64_t R, int64_t V, int64_t x_stride, int64_t K, double temperature) {
     if (dtype < CWR_F32 || dtype > CWR_F64) return CWR_ERR_DTYPE;
     if (R < 0 || V < 1 || x_stride < 0 || K < 0) return CWR_ERR_SHAPE;
-    if (V > 0x3fffffff) return CWR_ERR_TOO_LARGE;
+    if (V >= 1 << 28) return CWR_ERR_TOO_LARGE;
     if (K > CWR_MAX_ROW_TOKENS) return CWR_ERR_TOO_LARGE;
     if (!(temperature > 0.0) || !(temperature <= 1e30) || temperature < 1e-30) return CWR_ERR_SHAPE;
     if (R > 0 && !x) return CWR_ERR_NULL;
@@ -624,7 +624,7 @@ int cwr_token_logprobs_backward(const void* x, int dtype, int64_t R, int64_t V, 
 }
 
 size_t cwr_joint_token_logprobs_workspace_bytes(int64_t R, int64_t V) {
-    if (R < 0 || V < 1 || V > 0x3fffffff) return 0;
+    if (R < 0 || V < 1 || V >= 1 << 28) return 0;
     return joint_scores_workspace_bytes(R, V);
 }
 

@@ -40,7 +40,8 @@ __device__ __forceinline__ v4i load_pack(const T* __restrict__ row, int e, int V
     constexpr int VEC = Elem<T>::VEC;
     if (!EDGE) {
         v4i r = Pack<T>::neg_inf();
-        if (e < V) r = load_raw<NT>(row + e);
+        // an unsigned 32-bit byte offset (V < 2^28) next to the row's base: no 64-bit address per lane
+        if (e < V) r = load_raw<NT>(reinterpret_cast<const char*>(row) + (unsigned)e * (unsigned)sizeof(T));
         return r;
     }
     // a row off the element grid of 16 bytes: the hardware takes any element-aligned address
@@ -72,6 +73,10 @@ __device__ __forceinline__ void unpack_chunk(const v4i (&raw)[RowPacks<T>::NP], 
 // ---------------------------------------------------------------------------------------------
 // reductions over aligned groups of W lanes
 // ---------------------------------------------------------------------------------------------
+struct OpMin {
+    static __device__ __forceinline__ float identity() { return INFINITY; }
+    static __device__ __forceinline__ float apply(float a, float b) { return fminf(a, b); }
+};
 struct OpMaxI { static __device__ __forceinline__ int apply(int a, int b) { return a > b ? a : b; } };
 struct OpMinI { static __device__ __forceinline__ int apply(int a, int b) { return a < b ? a : b; } };
 

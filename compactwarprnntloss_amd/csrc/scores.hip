@@ -43,14 +43,14 @@ __device__ __forceinline__ TokenLogit fetch_token(const T* __restrict__ row, i64
     }
     return t;
 }
-__device__ __forceinline__ void write_token(const TokenLogit& t, i64 r, int j, int V, float m, float l2, const Temper& tp,
-                                            const ScoreArgs& a) {
+__device__ __forceinline__ void write_token(const TokenLogit& t, float lp, i64 r, int j, int V, const ScoreArgs& a) {
     if (j >= a.M) return;
-    float lp = 0.f;  // -1: no token
-    if ((unsigned)t.tok < (unsigned)V) lp = logprob(t.x, m, l2, tp);
-    else if (t.tok != -1) {
-        lp = __int_as_float(0x7fc00000);
-        if (a.status) raise_flag(a.status, CWR_FLAG_BAD_LABEL);
+    if ((unsigned)t.tok >= (unsigned)V) {
+        lp = 0.f;  // -1: no token
+        if (t.tok != -1) {
+            lp = __int_as_float(0x7fc00000);
+            if (a.status) raise_flag(a.status, CWR_FLAG_BAD_LABEL);
+        }
     }
     a.logprobs[r * a.M + j] = lp;
 }
@@ -111,8 +111,11 @@ __global__ __launch_bounds__(kWavesPerBlock * 64) void k_scores_group(const T* _
     const float l2 = row_l2(o, tp.c);
     if (ok && l == 0) write_row(r, o, l2, tp, a);
     if (ok) {
-        write_token(tok, r, l, V, o.m, l2, tp, a);
-        for (int j = l + G; j < a.M; j += G) write_token(fetch_token<T>(row, r, j, V, a), r, j, V, o.m, l2, tp, a);
+        write_token(tok, logprob(tok.x, o.m, l2, tp), r, l, V, a);
+        for (int j = l + G; j < a.M; j += G) {
+            const TokenLogit more = fetch_token<T>(row, r, j, V, a);
+            write_token(more, logprob(more.x, o.m, l2, tp), r, j, V, a);
+        }
     }
     if (a.K == 0) return;
     int key[kLaneElems];
@@ -198,15 +201,17 @@ __device__ __forceinline__ int list_compress(u64* list, int n, int K) {
     return n < K ? n : K;
 }
 
-// Largest bound found in a few steps that at least K of the lanes' values reach (as order_i32).
-__device__ __forceinline__ int kth_bound(int lane_best, int K) {
-    int lo = group_allreduce_i32<64, OpMinI>(lane_best);
-    const int top = group_allreduce_i32<64, OpMaxI>(lane_best);
-    unsigned span = (unsigned)top - (unsigned)lo;  // the bound lies in [lo, lo + span]
+// Largest bound found in a few steps that at least K of the lanes' values reach (as order_i32).  `top` is the
+// largest of them.  One compare per step on the vector unit, the search itself on the scalar unit.
+__device__ __forceinline__ int kth_bound(float lane_best, float top, int K) {
+    const int mine = order_i32(lane_best);
+    int lo = __builtin_amdgcn_readfirstlane(order_i32(group_allreduce<64, OpMin>(lane_best)));
+    // the bound lies in [lo, lo + span]
+    unsigned span = (unsigned)__builtin_amdgcn_readfirstlane(order_i32(top)) - (unsigned)lo;
     for (int step = 0; step < 20 && span > 0; ++step) {
         const unsigned half = (span + 1) >> 1;
         const int mid = (int)((unsigned)lo + half);
-        const int reach = __popcll(__ballot(lane_best >= mid));
+        const int reach = __popcll(__ballot(mine >= mid));
         if (reach >= K) {
             lo = mid;
             span -= half;
@@ -234,6 +239,18 @@ __device__ __forceinline__ void rank_append(Ranking& q, float f, int e, bool in)
     q.n += __popcll(takers);
 }
 
+// v[s] for a slot that differs between the lanes: selects of values (a choice between elements of the
+// array itself would put the array into memory)
+__device__ __forceinline__ float pick(bool second, float x, float y) { return second ? y : x; }
+__device__ __forceinline__ float pick16(const float (&v)[kLaneElems], int s) {
+    const bool s1 = s & 1, s2 = s & 2, s4 = s & 4, s8 = s & 8;
+    const float b0 = pick(s2, pick(s1, v[0], v[1]), pick(s1, v[2], v[3]));
+    const float b1 = pick(s2, pick(s1, v[4], v[5]), pick(s1, v[6], v[7]));
+    const float b2 = pick(s2, pick(s1, v[8], v[9]), pick(s1, v[10], v[11]));
+    const float b3 = pick(s2, pick(s1, v[12], v[13]), pick(s1, v[14], v[15]));
+    return pick(s8, pick(s4, b0, b1), pick(s4, b2, b3));
+}
+
 template <int VEC>
 __device__ __forceinline__ void rank_chunk(Ranking& q, const float (&v)[kLaneElems], float best, int e0, int V, int K) {
     if (__ballot(best >= q.floor_) == 0) return;
@@ -241,7 +258,11 @@ __device__ __forceinline__ void rank_chunk(Ranking& q, const float (&v)[kLaneEle
     // (about one lane in eight has any, hardly one has two)
     unsigned reach = 0;
 #pragma unroll
-    for (int s = 0; s < kLaneElems; ++s) reach |= v[s] >= q.floor_ ? 1u << s : 0u;
+    for (int s = kLaneElems - 1; s >= 0; --s)  // a compare, and its result shifted in as a carry
+        asm("v_cmp_le_f32 vcc, %1, %2\n\tv_addc_co_u32 %0, vcc, %0, %0, vcc"
+            : "+v"(reach)
+            : "v"(q.floor_), "v"(v[s])
+            : "vcc");
     for (;;) {
         const u64 some = __ballot(reach != 0);
         if (some == 0) break;
@@ -254,9 +275,7 @@ __device__ __forceinline__ void rank_chunk(Ranking& q, const float (&v)[kLaneEle
             }
         }
         const int s = __ffs((int)reach) - 1;  // -1: none left
-        float f = v[0];
-#pragma unroll
-        for (int i = 1; i < kLaneElems; ++i) f = i == s ? v[i] : f;
+        const float f = pick16(v, s);
         const int e = e0 + (s / VEC) * 64 * VEC + (s & (VEC - 1));
         rank_append(q, f, e, reach != 0 && (unsigned)e < (unsigned)V);
         reach &= reach - 1;
@@ -309,7 +328,7 @@ __global__ __launch_bounds__(64 * (NW > 1 ? NW : kWavesPerBlock), sizeof(T) == 2
             best = fmaxf(best, -INFINITY);
         }
         if (ch == first) {
-            const int lo = kth_bound(order_i32(best), a.K);
+            const int lo = kth_bound(best, top, a.K);
             q.floor_ = from_order_i32(lo);
             q.bound = (u64)((unsigned)lo ^ 0x80000000u) << 32;  // below every key of that value
         }
@@ -359,7 +378,19 @@ __global__ __launch_bounds__(64 * (NW > 1 ? NW : kWavesPerBlock), sizeof(T) == 2
     }
     const float l2 = row_l2(o, tp.c);
     if (lane == 0) write_row(r, o, l2, tp, a);
-    write_token(tok, r, lane, V, o.m, l2, tp, a);
+    if (a.M <= 32 && a.K <= 32) {  // one logarithm for both: tokens in the lower half of the wave, alternatives above
+        const int k = lane - 32;
+        const u64 key = k >= 0 && k < a.K ? q.list[k] : 0;
+        const TokenLogit both = {tok.tok, lane < 32 ? tok.x : key_value(key)};
+        const float lp = logprob(both.x, o.m, l2, tp);
+        if (lane < 32) write_token(both, lp, r, lane, V, a);
+        else if (k < a.K) {
+            a.top_index[r * a.K + k] = key_index(key);
+            a.top_logprobs[r * a.K + k] = lp;
+        }
+        return;
+    }
+    write_token(tok, logprob(tok.x, o.m, l2, tp), r, lane, V, a);
     if (lane < a.K) {
         const u64 key = q.list[lane];
         a.top_index[r * a.K + lane] = key_index(key);

@@ -345,7 +345,7 @@ int cwr_joint_backward(const void* h, const void* w, const float* bias, int dtyp
  * One read of x.  The reference has no counterpart: its callers run log_softmax on stored logits
  * (test/test.py:19-20).  The compact rows of a lattice are scored with tokens (blank, label).
  *   x            (R, V) of any cwr_dtype (64-bit entries are rounded to fp32 when read, as everywhere in
- *                this library), row r at x + r * x_stride, entries of a row adjacent; x_stride >= 0
+ *                this library), row r at x + r * x_stride, entries of a row adjacent; x_stride >= 0; V < 2^28
  *   tokens       (R, M) int32, M <= 64;  K <= 64, K <= V;  temperature > 0 and finite
  *   stat         (R, 4) fp32, 16-byte aligned, for cwr_token_logprobs_backward: row maximum, log2 of the scaled
  *                sum, entropy, 0;  NULL: not kept
