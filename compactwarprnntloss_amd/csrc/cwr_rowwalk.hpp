@@ -58,6 +58,25 @@ __device__ __forceinline__ v4i load_pack(const T* __restrict__ row, int e, int V
     return r;
 }
 
+// The packs of lane l of a group of G that make up the chunk whose first pack covers row elements [e0, ..).
+template <typename T, int G, bool EDGE, bool NT>
+__device__ __forceinline__ void load_chunk(const T* __restrict__ row, int e0, int l, int V, v4i (&raw)[RowPacks<T>::NP]) {
+    constexpr int VEC = RowPacks<T>::VEC, NP = RowPacks<T>::NP;
+    if (G == 64 && e0 >= 0 && e0 + 64 * kLaneElems <= V) {  // wholly inside the row: nothing to check
+        typedef v4i v4i_any __attribute__((aligned(2)));
+        const char* base = reinterpret_cast<const char*>(row) + (size_t)((unsigned)e0 * (unsigned)sizeof(T));
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const char* p = base + (unsigned)l * 16u + 1024u * i;
+            if (EDGE) raw[i] = *reinterpret_cast<const v4i_any*>(p);
+            else raw[i] = load_raw<NT>(p);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < NP; ++i) raw[i] = load_pack<T, EDGE, NT>(row, e0 + (i * G + l) * VEC, V);
+}
+
 template <typename T>
 __device__ __forceinline__ void unpack_chunk(const v4i (&raw)[RowPacks<T>::NP], float (&v)[kLaneElems]) {
     constexpr int VEC = RowPacks<T>::VEC;
@@ -73,12 +92,41 @@ __device__ __forceinline__ void unpack_chunk(const v4i (&raw)[RowPacks<T>::NP], 
 // ---------------------------------------------------------------------------------------------
 // reductions over aligned groups of W lanes
 // ---------------------------------------------------------------------------------------------
-struct OpMin {
-    static __device__ __forceinline__ float identity() { return INFINITY; }
-    static __device__ __forceinline__ float apply(float a, float b) { return fminf(a, b); }
-};
 struct OpMaxI { static __device__ __forceinline__ int apply(int a, int b) { return a > b ? a : b; } };
 struct OpMinI { static __device__ __forceinline__ int apply(int a, int b) { return a < b ? a : b; } };
+
+// A whole wave reduced by the vector unit alone: operations whose first operand comes through DPP, six of
+// them, the last lane then holds the result.  Written out because the compiler makes a move, a quieting
+// maximum and the operation out of each.  A DPP operand has to be two wait states old.
+#define CWR_WAVE_REDUCE(OP, v)                                                        \
+    asm("s_nop 1\n\t" OP " %0, %0, %0 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n\t" \
+        "s_nop 1\n\t" OP " %0, %0, %0 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n\t" \
+        "s_nop 1\n\t" OP " %0, %0, %0 row_half_mirror row_mask:0xf bank_mask:0xf\n\t"     \
+        "s_nop 1\n\t" OP " %0, %0, %0 row_mirror row_mask:0xf bank_mask:0xf\n\t"          \
+        "s_nop 1\n\t" OP " %0, %0, %0 row_bcast:15 row_mask:0xa bank_mask:0xf\n\t"        \
+        "s_nop 1\n\t" OP " %0, %0, %0 row_bcast:31 row_mask:0xc bank_mask:0xf\n\t"        \
+        "s_nop 1"                                                                     \
+        : "+v"(v))
+__device__ __forceinline__ float wave_max(float v) {
+    CWR_WAVE_REDUCE("v_max_f32_dpp", v);
+    return readlane_f32(v, 63);
+}
+__device__ __forceinline__ float wave_min(float v) {
+    CWR_WAVE_REDUCE("v_min_f32_dpp", v);
+    return readlane_f32(v, 63);
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    CWR_WAVE_REDUCE("v_add_f32_dpp", v);
+    return readlane_f32(v, 63);
+}
+template <int W> __device__ __forceinline__ float row_max(float v) {
+    if constexpr (W == 64) return wave_max(v);
+    else return group_allreduce<W, OpMax>(v);
+}
+template <int W> __device__ __forceinline__ float row_sum(float v) {
+    if constexpr (W == 64) return wave_sum(v);
+    else return group_allreduce<W, OpSum>(v);
+}
 
 template <int W, class Op>
 __device__ __forceinline__ int group_allreduce_i32(int v) {

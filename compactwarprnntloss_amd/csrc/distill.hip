@@ -62,20 +62,20 @@ __device__ __forceinline__ void teacher(const Entry& e, const Temper& tp, float&
     if (TAIL) {
         logq = e.t;
         q = fast_exp2(e.t * kLog2e);
-        Q = group_allreduce<G, OpSum>(q);
+        Q = row_sum<G>(q);
         return;
     }
     const float t = (float)((double)e.t * tp.inv);
-    const float mt = group_allreduce<G, OpMax>(t);
+    const float mt = row_max<G>(t);
     if (mt == -INFINITY) {  // an empty list, or one of -inf only
         q = t != t ? t : 0.f;
         logq = t;
-        Q = group_allreduce<G, OpSum>(q);
+        Q = row_sum<G>(q);
         return;
     }
     const float d = t - mt;
     const float ex = fast_exp2(d * kLog2e);
-    const float s = group_allreduce<G, OpSum>(ex);
+    const float s = row_sum<G>(ex);
     q = ex / s;
     logq = d - kLn2 * log2_of_sum(s);
     Q = s != s ? s : 1.f;
@@ -93,13 +93,13 @@ __device__ __forceinline__ void finish_row(i64 r, bool ok, int l, Online o, cons
     teacher<G, TAIL>(e, tp, q, logq, Q);
     const Online rest = o;
     if (TAIL) {
-        online_rebase(o, fmaxf(o.m, group_allreduce<G, OpMax>(e.x)), c);
-        o.s += group_allreduce<G, OpSum>(first ? fast_exp2(measure(e.x, anchor(o.m, c), c)) : 0.f);
+        online_rebase(o, fmaxf(o.m, row_max<G>(e.x)), c);
+        o.s += row_sum<G>(first ? fast_exp2(measure(e.x, anchor(o.m, c), c)) : 0.f);
     }
     const bool empty = o.m == -INFINITY && !(o.s != o.s);
     const float l2 = empty ? 0.f : log2_sum(o, c);
     const float term = q == 0.f || e.at < 0 ? 0.f : q * (logq - logprob(e.x, o.m, l2, tp));
-    float loss = group_allreduce<G, OpSum>(term);
+    float loss = row_sum<G>(term);
     float B = empty ? 0.f : Q * fast_exp2(-(l2 + ms_slip(o.m, c)));
     if (TAIL) {
         // the mass the list leaves in 64 bits: a list that holds nearly everything leaves a small difference
@@ -147,10 +147,7 @@ __global__ __launch_bounds__(64 * (NW > 1 ? NW : kWavesPerBlock)) void k_distill
     const int chunks = G < 64 ? 1 : (int)(((i64)V + off + CHUNK - 1) / CHUNK);
 
     v4i next[NP];
-    auto fetch = [&](int ch) {
-#pragma unroll
-        for (int i = 0; i < NP; ++i) next[i] = load_pack<T, EDGE, false>(row, ch * CHUNK + (i * G + l) * VEC - off, V);
-    };
+    auto fetch = [&](int ch) { load_chunk<T, G, EDGE, false>(row, ch * CHUNK - off, l, V, next); };
     if (first_chunk < chunks) fetch(first_chunk);
     const Entry e = load_entry<T>(row, rr, l, V, a.top, a.index, a.K);
     bool first = e.at >= 0;
@@ -176,14 +173,14 @@ __global__ __launch_bounds__(64 * (NW > 1 ? NW : kWavesPerBlock)) void k_distill
             for (int s = 0; s < kLaneElems; ++s) v[s] = (mine >> s) & 1 ? -INFINITY : v[s];
             wave_sync();
         }
-        const float top = group_allreduce<G, OpMax>(chunk_max(v));
+        const float top = row_max<G>(chunk_max(v));
         if (G < 64) o.m = top;
         else online_rebase(o, fmaxf(o.m, top), tp.c);
         float s, u;
         online_chunk<false>(v, o.m, tp.c, s, u);
         o.s += s;
     }
-    o.s = group_allreduce<G, OpSum>(o.s);
+    o.s = row_sum<G>(o.s);
     if (NW > 1) {
         if (lane == 0) parts[w] = o;
         __syncthreads();
@@ -302,8 +299,7 @@ __global__ __launch_bounds__(kWavesPerBlock * 64) void k_distill_grad(
     const int off = EDGE ? grid_offset(out) : 0;  // the stores decide: a load may start anywhere
     const int e0 = ch * CHUNK - off;              // row element of map place 0
     v4i raw[NP];
-#pragma unroll
-    for (int i = 0; i < NP; ++i) raw[i] = load_pack<T, EDGE, false>(row, e0 + (i * G + l) * VEC, V);
+    load_chunk<T, G, EDGE, false>(row, e0, l, V, raw);
     const Entry e = load_entry<T>(row, r, l, V, top, index, K);
     const float4 st = stat[r];
     float gt = go.p[r * go.stride] * go.scale / (float)tp.inv;

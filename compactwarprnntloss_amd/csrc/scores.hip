@@ -34,15 +34,16 @@ struct TokenLogit {
     int tok;
     float x;
 };
-template <typename T>
-__device__ __forceinline__ TokenLogit fetch_token(const T* __restrict__ row, i64 r, int j, int V, const ScoreArgs& a) {
+__device__ __forceinline__ TokenLogit fetch_token_index(i64 r, int j, const ScoreArgs& a) {
     TokenLogit t = {-1, 0.f};
-    if (j < a.M) {
-        t.tok = a.tokens[r * a.M + j];
-        if ((unsigned)t.tok < (unsigned)V) t.x = Elem<T>::to_f32(row[t.tok]);
-    }
+    if (j < a.M) t.tok = a.tokens[r * a.M + j];
     return t;
 }
+template <typename T>
+__device__ __forceinline__ void fetch_token_logit(TokenLogit& t, const T* __restrict__ row, int V) {
+    if ((unsigned)t.tok < (unsigned)V) t.x = Elem<T>::to_f32(row[t.tok]);
+}
+
 __device__ __forceinline__ void write_token(const TokenLogit& t, float lp, i64 r, int j, int V, const ScoreArgs& a) {
     if (j >= a.M) return;
     if ((unsigned)t.tok >= (unsigned)V) {
@@ -97,23 +98,24 @@ __global__ __launch_bounds__(kWavesPerBlock * 64) void k_scores_group(const T* _
     const bool ok = r < R;
     const T* row = x + (ok ? r : R - 1) * stride;
     const int off = EDGE ? grid_offset(row) : 0;
+    TokenLogit tok = fetch_token_index(ok ? r : R - 1, l, a);
     v4i raw[NP];
-#pragma unroll
-    for (int i = 0; i < NP; ++i) raw[i] = load_pack<T, EDGE, true>(row, (i * G + l) * VEC - off, V);
-    const TokenLogit tok = fetch_token<T>(row, ok ? r : R - 1, l, V, a);
+    load_chunk<T, G, EDGE, true>(row, -off, l, V, raw);
+    fetch_token_logit<T>(tok, row, V);
     float v[kLaneElems];
     unpack_chunk<T>(raw, v);
     Online o;
-    o.m = group_allreduce<G, OpMax>(chunk_max(v));
+    o.m = row_max<G>(chunk_max(v));
     online_chunk<true>(v, o.m, tp.c, o.s, o.u);
-    o.s = group_allreduce<G, OpSum>(o.s);
-    o.u = group_allreduce<G, OpSum>(o.u);
+    o.s = row_sum<G>(o.s);
+    o.u = row_sum<G>(o.u);
     const float l2 = row_l2(o, tp.c);
     if (ok && l == 0) write_row(r, o, l2, tp, a);
     if (ok) {
         write_token(tok, logprob(tok.x, o.m, l2, tp), r, l, V, a);
         for (int j = l + G; j < a.M; j += G) {
-            const TokenLogit more = fetch_token<T>(row, r, j, V, a);
+            TokenLogit more = fetch_token_index(r, j, a);
+            fetch_token_logit<T>(more, row, V);
             write_token(more, logprob(more.x, o.m, l2, tp), r, j, V, a);
         }
     }
@@ -205,7 +207,7 @@ __device__ __forceinline__ int list_compress(u64* list, int n, int K) {
 // largest of them.  One compare per step on the vector unit, the search itself on the scalar unit.
 __device__ __forceinline__ int kth_bound(float lane_best, float top, int K) {
     const int mine = order_i32(lane_best);
-    int lo = __builtin_amdgcn_readfirstlane(order_i32(group_allreduce<64, OpMin>(lane_best)));
+    int lo = __builtin_amdgcn_readfirstlane(order_i32(wave_min(lane_best)));
     // the bound lies in [lo, lo + span]
     unsigned span = (unsigned)__builtin_amdgcn_readfirstlane(order_i32(top)) - (unsigned)lo;
     for (int step = 0; step < 20 && span > 0; ++step) {
@@ -242,7 +244,7 @@ __device__ __forceinline__ void rank_append(Ranking& q, float f, int e, bool in)
 // v[s] for a slot that differs between the lanes: selects of values (a choice between elements of the
 // array itself would put the array into memory)
 __device__ __forceinline__ float pick(bool second, float x, float y) { return second ? y : x; }
-__device__ __forceinline__ float pick16(const float (&v)[kLaneElems], int s) {
+__device__ __forceinline__ float pick16(const float (&v)[kLaneElems], unsigned s) {
     const bool s1 = s & 1, s2 = s & 2, s4 = s & 4, s8 = s & 8;
     const float b0 = pick(s2, pick(s1, v[0], v[1]), pick(s1, v[2], v[3]));
     const float b1 = pick(s2, pick(s1, v[4], v[5]), pick(s1, v[6], v[7]));
@@ -274,9 +276,9 @@ __device__ __forceinline__ void rank_chunk(Ranking& q, const float (&v)[kLaneEle
                 q.floor_ = key_value(q.bound);
             }
         }
-        const int s = __ffs((int)reach) - 1;  // -1: none left
+        const unsigned s = (unsigned)(__ffs((int)reach) - 1) & 15u;  // (none left: any)
         const float f = pick16(v, s);
-        const int e = e0 + (s / VEC) * 64 * VEC + (s & (VEC - 1));
+        const int e = e0 + (int)((s / VEC) * 64 * VEC + (s & (VEC - 1)));
         rank_append(q, f, e, reach != 0 && (unsigned)e < (unsigned)V);
         reach &= reach - 1;
         wave_sync();
@@ -303,19 +305,16 @@ __global__ __launch_bounds__(64 * (NW > 1 ? NW : kWavesPerBlock), sizeof(T) == 2
     Online o = {-INFINITY, 0.f, 0.f};
     Ranking q = {lists[w], 0, 0, -INFINITY};
     v4i next[NP];
-    auto fetch = [&](int ch) {
-#pragma unroll
-        for (int i = 0; i < NP; ++i)
-            next[i] = load_pack<T, EDGE, true>(row, ch * CHUNK + (i * 64 + lane) * VEC - off, V);
-    };
+    auto fetch = [&](int ch) { load_chunk<T, 64, EDGE, true>(row, ch * CHUNK - off, lane, V, next); };
+    TokenLogit tok = fetch_token_index(r, lane, a);
     if (first < chunks) fetch(first);
-    const TokenLogit tok = fetch_token<T>(row, r, lane, V, a);
+    fetch_token_logit<T>(tok, row, V);
     for (int ch = first; ch < chunks; ch += NW) {
         float v[kLaneElems];
         unpack_chunk<T>(next, v);
         if (ch + NW < chunks) fetch(ch + NW);
         float best = chunk_max(v);
-        const float top = group_allreduce<64, OpMax>(best);
+        const float top = wave_max(best);
         online_rebase(o, fmaxf(o.m, top), tp.c);
         float s, u;
         online_chunk<true>(v, o.m, tp.c, s, u);
@@ -336,8 +335,8 @@ __global__ __launch_bounds__(64 * (NW > 1 ? NW : kWavesPerBlock), sizeof(T) == 2
     }
 
     // the lanes' sums, then the waves'
-    o.s = group_allreduce<64, OpSum>(o.s);
-    o.u = group_allreduce<64, OpSum>(o.u);
+    o.s = wave_sum(o.s);
+    o.u = wave_sum(o.u);
     if (a.K > 0) q.n = list_compress(q.list, q.n, a.K);
     if (NW > 1) {
         if (lane == 0) parts[w] = o;
@@ -449,8 +448,7 @@ __global__ __launch_bounds__(kWavesPerBlock * 64) void k_scores_grad(const T* __
     const int off = EDGE ? grid_offset(out) : 0;  // the stores decide: a load may start anywhere
     const int e0 = ch * CHUNK - off;              // row element of map place 0
     v4i raw[NP];
-#pragma unroll
-    for (int i = 0; i < NP; ++i) raw[i] = load_pack<T, EDGE, true>(row, e0 + (i * G + l) * VEC, V);
+    load_chunk<T, G, EDGE, true>(row, e0, l, V, raw);
 
     // the row's entries and their incoming gradients
     const int n = a.M + a.K;
@@ -488,7 +486,7 @@ __global__ __launch_bounds__(kWavesPerBlock * 64) void k_scores_grad(const T* __
             gin[e] = gr;
         }
     }
-    wsum = group_allreduce<G, OpSum>(wsum);
+    wsum = row_sum<G>(wsum);
 
     const float4 st = a.stat[r];
     const float m = st.x, l2 = st.y;
