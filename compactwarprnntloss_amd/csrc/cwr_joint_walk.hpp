@@ -1,6 +1,7 @@
 // How the output-layer kernels walk the product logits[r, v] = sum_k h[r, k] * W[v, k] + bias[v]: the two
 // tilings (data rows streamed through LDS, or resident in registers) hand every finished tile of
-// fp32 accumulators to their caller.
+// fp32 accumulators to their caller.  In a 32x32 block of accumulators a lane holds 16 vocabulary entries
+// (acc_row) of the data row lane % 32; with SWAP it is the other way round, 16 data rows of one entry.
 #pragma once
 
 #include "cwr_device.hpp"
@@ -46,7 +47,7 @@ template <typename T> struct StreamLds {
     float bias[2][kJN];  // what the accumulators of a tile start from
 };
 
-template <typename T, typename TB, typename TileFn>
+template <typename T, typename TB, bool SWAP = false, typename TileFn>
 __device__ __forceinline__ void walk_streaming(const T* __restrict__ h, const T* __restrict__ W,
                                                const TB* __restrict__ bias, i64 R, int H, int V, i64 row0,
                                                StreamLds<T>& lds, TileFn&& tile) {
@@ -120,7 +121,8 @@ __device__ __forceinline__ void walk_streaming(const T* __restrict__ h, const T*
             for (int mv = 0; mv < 2; ++mv)
 #pragma unroll
                 for (int b4 = 0; b4 < 4; ++b4) {
-                    const float4 bq = *reinterpret_cast<const float4*>(&s_bias[vt & 1][64 * wv + 32 * mv + 8 * b4 + 4 * hf]);
+                    float4 bq = *reinterpret_cast<const float4*>(&s_bias[vt & 1][64 * wv + 32 * mv + 8 * b4 + 4 * hf]);
+                    if (SWAP) bq.x = bq.y = bq.z = bq.w = s_bias[vt & 1][64 * wv + 32 * mv + l32];
 #pragma unroll
                     for (int nd = 0; nd < 4; ++nd) {
                         acc[mv][nd][4 * b4 + 0] = bq.x; acc[mv][nd][4 * b4 + 1] = bq.y;
@@ -143,7 +145,8 @@ __device__ __forceinline__ void walk_streaming(const T* __restrict__ h, const T*
 #pragma unroll
             for (int mv = 0; mv < 2; ++mv)
 #pragma unroll
-                for (int nd = 0; nd < 4; ++nd) acc[mv][nd] = Mfma<T>::mac(fa[mv], fb[nd], acc[mv][nd]);
+                for (int nd = 0; nd < 4; ++nd)
+                    acc[mv][nd] = SWAP ? Mfma<T>::mac(fb[nd], fa[mv], acc[mv][nd]) : Mfma<T>::mac(fa[mv], fb[nd], acc[mv][nd]);
         }
         if (it + 1 < iters) stage(buf ^ 1, next);
         __syncthreads();
@@ -208,8 +211,8 @@ __device__ __forceinline__ void load_resident_rows(const T* __restrict__ h, i64 
 // (what the caller still has to do about its rows: loads issued here queue up BEHIND the rows',
 // whatever the caller asked for earlier is served before them), and the first tile starts as
 // soon as the first fragments are there.
-template <typename T, int ND, int KS, int NMV, int WAVES, int RK, bool D2, typename LoadRows, typename TB,
-          typename AfterIssue, typename TileFn>
+template <typename T, int ND, int KS, int NMV, int WAVES, int RK, bool D2, bool SWAP = false, typename LoadRows,
+          typename TB, typename AfterIssue, typename TileFn>
 __device__ __forceinline__ void walk_resident(LoadRows&& load_rows, const T* __restrict__ W,
                                               const TB* __restrict__ bias, int V, ResLds<T, NMV, RK>& lds,
                                               AfterIssue&& after_issue, TileFn&& tile) {
@@ -274,7 +277,8 @@ __device__ __forceinline__ void walk_resident(LoadRows&& load_rows, const T* __r
         for (int mv = 0; mv < NMV; ++mv)
 #pragma unroll
             for (int b4 = 0; b4 < 4; ++b4) {
-                const float4 bq = *reinterpret_cast<const float4*>(&s_bias[vt & 1][32 * mv + 8 * b4 + 4 * hf]);
+                float4 bq = *reinterpret_cast<const float4*>(&s_bias[vt & 1][32 * mv + 8 * b4 + 4 * hf]);
+                if (SWAP) bq.x = bq.y = bq.z = bq.w = s_bias[vt & 1][32 * mv + l32];
 #pragma unroll
                 for (int nd = 0; nd < ND; ++nd) {
                     acc[mv][nd][4 * b4 + 0] = bq.x; acc[mv][nd][4 * b4 + 1] = bq.y;
@@ -309,7 +313,8 @@ __device__ __forceinline__ void walk_resident(LoadRows&& load_rows, const T* __r
                 for (int mv = 0; mv < NMV; ++mv)
 #pragma unroll
                     for (int nd = 0; nd < ND; ++nd)
-                        acc[mv][nd] = Mfma<T>::mac(fa[mv], hreg[nd][kc * (RK / 16) + ks], acc[mv][nd]);
+                        acc[mv][nd] = SWAP ? Mfma<T>::mac(hreg[nd][kc * (RK / 16) + ks], fa[mv], acc[mv][nd])
+                                           : Mfma<T>::mac(fa[mv], hreg[nd][kc * (RK / 16) + ks], acc[mv][nd]);
                 __builtin_amdgcn_sched_barrier(0);
             }
             {

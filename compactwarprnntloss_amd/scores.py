@@ -178,7 +178,7 @@ def joint_token_logprobs(h: torch.Tensor, weight: torch.Tensor, bias: Optional[t
     """token_logprobs of the logits h @ weight.T + bias without storing them: h (R, H) joint rows (from
     compact_join, or one row per hypothesis of a search), weight (V, H), both fp16 or both bf16 with H a
     multiple of 32; bias (V,) in the same type or fp32, or None.  The product runs on the matrix cores with
-    fp32 accumulation and is scored from fp32, a block of rows at a time (at most 128 MiB, or 4096 rows).
+    fp32 accumulation and is scored from fp32, a block of rows at a time (256 MiB of workspace at most, or 4096 rows).
 
     For a teacher's pass over a lattice and for the steps of a search: the scores carry no gradient, and a
     call that would need one is refused."""
