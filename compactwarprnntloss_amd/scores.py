@@ -66,20 +66,23 @@ def _check_rows(x: torch.Tensor, temperature: float):
         raise RuntimeError("temperature must be positive and finite")
 
 
-def _check_tokens(tokens: Optional[torch.Tensor], R: int, device) -> Optional[torch.Tensor]:
+def _check_tokens(tokens: Optional[torch.Tensor], R: int, device) -> int:
+    """Tokens per row M of a (R,) or (R, M) tensor of tokens, 0 for None."""
     if tokens is None:
-        return None
+        return 0
     if tokens.device != device:
         raise RuntimeError("tokens must be on the device of x")
     if tokens.dtype != torch.int32:
         raise RuntimeError("tokens must be torch::ScalarType::Int")
-    if tokens.dim() not in (1, 2) or tokens.size(0) != R:
+    dims = tokens.dim()
+    if dims not in (1, 2) or tokens.size(0) != R:
         raise RuntimeError("tokens must be (R,) or (R, M)")
     if not tokens.is_contiguous():
         raise RuntimeError("tokens must be contiguous")
-    if tokens.dim() == 2 and not 1 <= tokens.size(1) <= MAX_ROW_TOKENS:
+    M = tokens.size(1) if dims == 2 else 1
+    if not 1 <= M <= MAX_ROW_TOKENS:
         raise RuntimeError(f"tokens must hold 1 to {MAX_ROW_TOKENS} tokens per row")
-    return tokens.view(R, -1) if R else tokens.view(0, tokens.size(1) if tokens.dim() == 2 else 1)
+    return M
 
 
 def _check_top_k(top_k: int, V: int) -> int:
@@ -92,20 +95,26 @@ def _new_status(device) -> torch.Tensor:
     return torch.zeros(4, dtype=torch.int32, device=device)
 
 
-def _run_scores(x, tokens, top_k, want_entropy, temperature, status, keep):
-    """Binding of cwr_token_logprobs: (logprobs, entropy, lse, top_logprobs, top_index, stat)."""
-    R, V = x.shape
-    dev = x.device
-    M = tokens.size(1) if tokens is not None else 0
+def _score_buffers(R: int, M: int, top_k: int, want_entropy: bool, dev):
+    """(logprobs, entropy, lse, top_logprobs, top_index) to be written.  Sizes as separate arguments: half a
+    microsecond less per tensor than a tuple, which a step of a search feels."""
     f32 = torch.float32
-    logprobs = torch.empty((R, M), dtype=f32, device=dev) if M else None
+    logprobs = torch.empty(R, M, dtype=f32, device=dev) if M else None
     entropy = torch.empty(R, dtype=f32, device=dev) if want_entropy else None
     lse = torch.empty(R, dtype=f32, device=dev)
     top = index = None
     if top_k:
-        top = torch.empty((R, top_k), dtype=f32, device=dev)
-        index = torch.empty((R, top_k), dtype=torch.int32, device=dev)
-    stat = torch.empty((R, 4), dtype=f32, device=dev) if keep else None
+        top = torch.empty(R, top_k, dtype=f32, device=dev)
+        index = torch.empty(R, top_k, dtype=torch.int32, device=dev)
+    return logprobs, entropy, lse, top, index
+
+
+def _run_scores(x, tokens, M, top_k, want_entropy, temperature, status, keep):
+    """Binding of cwr_token_logprobs: (logprobs, entropy, lse, top_logprobs, top_index, stat)."""
+    R, V = x.shape
+    dev = x.device
+    logprobs, entropy, lse, top, index = _score_buffers(R, M, top_k, want_entropy, dev)
+    stat = torch.empty(R, 4, dtype=torch.float32, device=dev) if keep else None
     _call("cwr_token_logprobs", dev, x.data_ptr(), _DTYPES[x.dtype], R, V, x.stride(0), _ptr(tokens), M, top_k,
           temperature, _ptr(stat), _ptr(logprobs), _ptr(entropy), lse.data_ptr(), _ptr(top), _ptr(index), _ptr(status))
     return logprobs, entropy, lse, top, index, stat
@@ -113,12 +122,12 @@ def _run_scores(x, tokens, top_k, want_entropy, temperature, status, keep):
 
 class _TokenScores(torch.autograd.Function):
     @staticmethod
-    def forward(ctx: Any, x, tokens, top_k, want_entropy, temperature, status):
-        logprobs, entropy, lse, top, index, stat = _run_scores(x, tokens, top_k, want_entropy, temperature, status, True)
+    def forward(ctx: Any, x, tokens, M, top_k, want_entropy, temperature, status):
+        logprobs, entropy, lse, top, index, stat = _run_scores(x, tokens, M, top_k, want_entropy, temperature, status, True)
         if index is not None:
             ctx.mark_non_differentiable(index)
         ctx.set_materialize_grads(False)
-        ctx.temperature = temperature
+        ctx.temperature, ctx.M = temperature, M
         ctx.save_for_backward(x, tokens, index, stat)
         return logprobs, entropy, lse, top, index
 
@@ -130,9 +139,9 @@ class _TokenScores(torch.autograd.Function):
         grads = [g if g is None else _rows_f32(g) for g in (g_logprobs, g_entropy, g_lse, g_top)]
         dx = torch.empty((R, V), dtype=x.dtype, device=x.device)
         _call("cwr_token_logprobs_backward", x.device, x.data_ptr(), _DTYPES[x.dtype], R, V, x.stride(0), _ptr(tokens),
-              tokens.size(1) if tokens is not None else 0, _ptr(index), index.size(1) if index is not None else 0,
+              ctx.M, _ptr(index), index.size(1) if index is not None else 0,
               ctx.temperature, stat.data_ptr(), *[_ptr(g) for g in grads], dx.data_ptr())
-        return dx, None, None, None, None, None
+        return dx, None, None, None, None, None, None
 
 
 def _rows_f32(g: torch.Tensor) -> torch.Tensor:
@@ -158,13 +167,13 @@ def token_logprobs(x: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, to
     temperature = float(temperature)
     _check_rows(x, temperature)
     R, V = x.shape
-    rows = _check_tokens(tokens, R, x.device)
+    M = _check_tokens(tokens, R, x.device)
     status = _new_status(x.device) if validate else None
     top_k = _check_top_k(top_k, V)
     if x.requires_grad and torch.is_grad_enabled():
-        logprobs, ent, lse, top, index = _TokenScores.apply(x, rows, top_k, bool(entropy), temperature, status)
+        logprobs, ent, lse, top, index = _TokenScores.apply(x, tokens, M, top_k, bool(entropy), temperature, status)
     else:
-        logprobs, ent, lse, top, index, _ = _run_scores(x, rows, top_k, bool(entropy), temperature, status, False)
+        logprobs, ent, lse, top, index, _ = _run_scores(x, tokens, M, top_k, bool(entropy), temperature, status, False)
     if validate:
         _raise_on_status(status, "token_logprobs")
     if tokens is not None and tokens.dim() == 1:
@@ -202,22 +211,14 @@ def joint_token_logprobs(h: torch.Tensor, weight: torch.Tensor, bias: Optional[t
     if torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         raise RuntimeError("joint_token_logprobs has no gradient: call it under torch.no_grad(), or use "
                            "token_logprobs on stored logits")
-    rows = _check_tokens(tokens, R, dev)
+    M = _check_tokens(tokens, R, dev)
     top_k = _check_top_k(top_k, V)
     status = _new_status(dev) if validate else None
-    M = rows.size(1) if rows is not None else 0
-    f32 = torch.float32
-    logprobs = torch.empty((R, M), dtype=f32, device=dev) if M else None
-    ent = torch.empty(R, dtype=f32, device=dev) if entropy else None
-    lse = torch.empty(R, dtype=f32, device=dev)
-    top = index = None
-    if top_k:
-        top = torch.empty((R, top_k), dtype=f32, device=dev)
-        index = torch.empty((R, top_k), dtype=torch.int32, device=dev)
+    logprobs, ent, lse, top, index = _score_buffers(R, M, top_k, entropy, dev)
     nbytes = _lib.load().cwr_joint_token_logprobs_workspace_bytes(R, V)
     work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _call("cwr_joint_token_logprobs", dev, h.data_ptr(), weight.data_ptr(), _ptr(bias),
-          _DTYPES[bias.dtype] if bias is not None else _lib.F32, _DTYPES[h.dtype], R, H, V, _ptr(rows), M, top_k,
+          _DTYPES[bias.dtype] if bias is not None else _lib.F32, _DTYPES[h.dtype], R, H, V, _ptr(tokens), M, top_k,
           temperature, _ptr(logprobs), _ptr(ent), lse.data_ptr(), _ptr(top), _ptr(index), work.data_ptr(), nbytes,
           _ptr(status))
     if validate:

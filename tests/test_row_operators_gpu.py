@@ -55,7 +55,7 @@ def test_teacher_to_student_training_step(tail):
 
 def _steps(x, tok, top, idx, h, w):
     """One forward and backward pass of each operator through the entry points, no autograd graph of x alive."""
-    r = scores._run_scores(x, tok, 4, True, 1.0, None, True)
+    r = scores._run_scores(x, tok, 2, 4, True, 1.0, None, True)
     leaf = x.detach().requires_grad_(True)
     out = pkg.token_logprobs(leaf, tok, top_k=4, entropy=True)
     d1, = torch.autograd.grad([out.logprobs, out.entropy, out.top_logprobs], leaf,
