@@ -4,8 +4,7 @@
 // A chunk is 16 G elements held by G consecutive lanes: pack i of lane l covers elements
 // ((i G + l) VEC - off) .. + VEC, so that the lanes of one load instruction touch consecutive
 // 16-byte packs.  `off` shifts the packs of a row that does not start on a 16-byte boundary back to
-// that grid; the packs at its two ends, which then stick out of the row, are read element by element
-// and never touch memory outside the row.
+// that grid; the packs at its two ends then stick out of the row.
 #pragma once
 
 #include "cwr_device.hpp"
@@ -33,29 +32,46 @@ template <typename T> __device__ __forceinline__ int grid_offset(const T* p) {
     return (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
 }
 
-// The pack of row elements [e, e + VEC); elements outside [0, V) come back as -inf.  EDGE = false: rows
-// are whole packs on the 16-byte grid, a pack is inside the row or outside it.
+// The pack of row elements [e, e + VEC).  EDGE = false: rows are whole packs on the 16-byte grid; a pack outside
+// the row comes back as -inf.  EDGE = true: a pack that sticks out of the row is read whole where it lies on the
+// grid (its 16 bytes hold an element of the row, so they are memory of the same allocation; what is not
+// the row's is struck out by mask_chunk or never used), and element by element where it does not.
 template <typename T, bool EDGE, bool NT>
 __device__ __forceinline__ v4i load_pack(const T* __restrict__ row, int e, int V) {
     constexpr int VEC = Elem<T>::VEC;
+    v4i r = Pack<T>::neg_inf();
     if (!EDGE) {
-        v4i r = Pack<T>::neg_inf();
         // an unsigned 32-bit byte offset (V < 2^28) next to the row's base: no 64-bit address per lane
         if (e < V) r = load_raw<NT>(reinterpret_cast<const char*>(row) + (unsigned)e * (unsigned)sizeof(T));
         return r;
     }
     // a row off the element grid of 16 bytes: the hardware takes any element-aligned address
     typedef v4i v4i_any __attribute__((aligned(2)));
-    if (e >= 0 && e + VEC <= V) return *reinterpret_cast<const v4i_any*>(row + e);
-    PackT<T, VEC> p;
-    const v4i none = Pack<T>::neg_inf();
-    __builtin_memcpy(&p, &none, 16);
+    const bool some = e + VEC > 0 && e < V, whole = e >= 0 && e + VEC <= V;
+    const bool grid = (reinterpret_cast<uintptr_t>(row + e) & 15) == 0;
+    if (whole || (some && grid)) {
+        r = *reinterpret_cast<const v4i_any*>(row + e);
+    } else if (some) {
+        PackT<T, VEC> p;
+        __builtin_memcpy(&p, &r, 16);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j)
-        if ((unsigned)(e + j) < (unsigned)V) p.e[j] = row[e + j];
-    v4i r;
-    __builtin_memcpy(&r, &p, 16);
+        for (int j = 0; j < VEC; ++j)
+            if ((unsigned)(e + j) < (unsigned)V) p.e[j] = row[e + j];
+        __builtin_memcpy(&r, &p, 16);
+    }
     return r;
+}
+
+// Elements of a chunk that lie outside the row become -inf (EDGE rows; the others' packs are whole).
+template <typename T, int G, bool EDGE>
+__device__ __forceinline__ void mask_chunk(float (&v)[kLaneElems], int e0, int l, int V) {
+    constexpr int VEC = Elem<T>::VEC;
+    if (!EDGE || (G == 64 && e0 >= 0 && e0 + 64 * kLaneElems <= V)) return;
+#pragma unroll
+    for (int s = 0; s < kLaneElems; ++s) {
+        const int e = e0 + ((s / VEC) * G + l) * VEC + (s & (VEC - 1));
+        v[s] = (unsigned)e < (unsigned)V ? v[s] : -INFINITY;
+    }
 }
 
 // The packs of lane l of a group of G that make up the chunk whose first pack covers row elements [e0, ..).

@@ -156,6 +156,7 @@ __global__ __launch_bounds__(64 * (NW > 1 ? NW : kWavesPerBlock)) void k_distill
     for (int ch = first_chunk; ch < chunks; ch += NW) {
         float v[kLaneElems];
         unpack_chunk<T>(next, v);
+        mask_chunk<T, G, EDGE>(v, ch * CHUNK - off, l, V);
         if (G == 64 && ch + NW < chunks) fetch(ch + NW);
         if (TAIL) {
             marks[w][lane] = 0;

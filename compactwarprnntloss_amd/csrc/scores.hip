@@ -104,6 +104,7 @@ __global__ __launch_bounds__(kWavesPerBlock * 64) void k_scores_group(const T* _
     fetch_token_logit<T>(tok, row, V);
     float v[kLaneElems];
     unpack_chunk<T>(raw, v);
+    mask_chunk<T, G, EDGE>(v, -off, l, V);
     Online o;
     o.m = row_max<G>(chunk_max(v));
     online_chunk<true>(v, o.m, tp.c, o.s, o.u);
@@ -312,6 +313,7 @@ __global__ __launch_bounds__(64 * (NW > 1 ? NW : kWavesPerBlock), sizeof(T) == 2
     for (int ch = first; ch < chunks; ch += NW) {
         float v[kLaneElems];
         unpack_chunk<T>(next, v);
+        mask_chunk<T, 64, EDGE>(v, ch * CHUNK - off, lane, V);
         if (ch + NW < chunks) fetch(ch + NW);
         float best = chunk_max(v);
         const float top = wave_max(best);
