@@ -31,79 +31,123 @@ struct DistillArgs {
     int* status;   // may be null
 };
 
-// A lane's entry of the list: x its student logit, t the teacher's value
+// An entry of the list: x its student logit, t the teacher's value.  Lane l of a group of G holds entries
+// l, l + G, ..: E of them, so that a long list does not widen the group a short row needs.
 struct Entry {
     int at;  // -1: none
     float t, x;
-    bool bad;
 };
 
-template <typename T>
-__device__ __forceinline__ Entry load_entry(const T* __restrict__ row, i64 r, int l, int V, const float* __restrict__ top,
-                                            const int* __restrict__ index, int K) {
-    Entry e = {-1, -INFINITY, -INFINITY, false};
-    if (l < K) {
-        const int at = index[r * K + l];
-        const float t = top[r * K + l];
-        if ((unsigned)at < (unsigned)V) {
-            e.at = at;
-            e.t = t;
-            e.x = Elem<T>::to_f32(row[at]);
-        } else {
-            e.bad = at != -1;
+// returns whether an index was out of range
+template <typename T, int G, int E>
+__device__ __forceinline__ bool load_entries(const T* __restrict__ row, i64 r, int l, int V, const float* __restrict__ top,
+                                             const int* __restrict__ index, int K, Entry (&e)[E]) {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        e[i].at = -1;
+        e[i].t = -INFINITY;
+        if (l + i * G < K) {
+            e[i].at = index[r * K + l + i * G];
+            e[i].t = top[r * K + l + i * G];
         }
     }
-    return e;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        e[i].x = -INFINITY;
+        if ((unsigned)e[i].at < (unsigned)V) {
+            e[i].x = Elem<T>::to_f32(row[e[i].at]);
+        } else {
+            bad |= e[i].at != -1;
+            e[i].at = -1;
+            e[i].t = -INFINITY;
+        }
+    }
+    return bad;
 }
 
-// The teacher's probabilities of a row: q of this lane's entry, its logarithm, and the mass Q of the list.
-template <int G, bool TAIL>
-__device__ __forceinline__ void teacher(const Entry& e, const Temper& tp, float& q, float& logq, float& Q) {
+// The teacher's probabilities of a row: q of this lane's entries, their logarithms, and the mass Q of the list.
+template <int G, bool TAIL, int E>
+__device__ __forceinline__ void teacher(const Entry (&e)[E], const Temper& tp, float (&q)[E], float (&logq)[E], float& Q) {
+    float sum = 0.f;
     if (TAIL) {
-        logq = e.t;
-        q = fast_exp2(e.t * kLog2e);
-        Q = row_sum<G>(q);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            logq[i] = e[i].t;
+            q[i] = fast_exp2(e[i].t * kLog2e);
+            sum += q[i];
+        }
+        Q = row_sum<G>(sum);
         return;
     }
-    const float t = (float)((double)e.t * tp.inv);
-    const float mt = row_max<G>(t);
-    if (mt == -INFINITY) {  // an empty list, or one of -inf only
-        q = t != t ? t : 0.f;
-        logq = t;
-        Q = row_sum<G>(q);
+    float mt = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        logq[i] = (float)((double)e[i].t * tp.inv);
+        mt = fmaxf(mt, logq[i]);
+    }
+    mt = row_max<G>(mt);
+    if (mt == -INFINITY) {  // an empty list, or one of -inf only (or NaN)
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            q[i] = logq[i] != logq[i] ? logq[i] : 0.f;
+            sum += q[i];
+        }
+        Q = row_sum<G>(sum);
         return;
     }
-    const float d = t - mt;
-    const float ex = fast_exp2(d * kLog2e);
-    const float s = row_sum<G>(ex);
-    q = ex / s;
-    logq = d - kLn2 * log2_of_sum(s);
-    Q = s != s ? s : 1.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        logq[i] -= mt;
+        q[i] = fast_exp2(logq[i] * kLog2e);
+        sum += q[i];
+    }
+    sum = row_sum<G>(sum);
+    const float logs = kLn2 * log2_of_sum(sum);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        q[i] /= sum;
+        logq[i] -= logs;
+    }
+    Q = sum != sum ? sum : 1.f;
 }
 
 constexpr float kPoisoned = INFINITY;  // in place of a row's log2 sum: an index outside the vocabulary was met
 
 // Everything behind the sums of a row, by the G lanes that share it.  o: the sums over the whole row, or with
-// TAIL over the entries outside the list; first: this lane's entry is the one of its index that counts
-template <int G, bool TAIL>
-__device__ __forceinline__ void finish_row(i64 r, bool ok, int l, Online o, const Entry& e, bool first, const Temper& tp,
-                                           const DistillArgs& a) {
+// TAIL over the entries outside the list; first: bit i, this lane's entry i is the one of its index that counts
+template <int G, bool TAIL, int E>
+__device__ __forceinline__ void finish_row(i64 r, bool ok, int l, Online o, const Entry (&e)[E], unsigned first, bool bad,
+                                           const Temper& tp, const DistillArgs& a) {
     const float c = tp.c;
-    float q, logq, Q;
-    teacher<G, TAIL>(e, tp, q, logq, Q);
+    float q[E], logq[E], Q;
+    teacher<G, TAIL, E>(e, tp, q, logq, Q);
     const Online rest = o;
     if (TAIL) {
-        online_rebase(o, fmaxf(o.m, row_max<G>(e.x)), c);
-        o.s += row_sum<G>(first ? fast_exp2(measure(e.x, anchor(o.m, c), c)) : 0.f);
+        float mx = e[0].x;
+#pragma unroll
+        for (int i = 1; i < E; ++i) mx = fmaxf(mx, e[i].x);
+        online_rebase(o, fmaxf(o.m, row_max<G>(mx)), c);
+        const Anchor anc = anchor(o.m, c);
+        float listed = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) listed += (first >> i) & 1 ? fast_exp2(measure(e[i].x, anc, c)) : 0.f;
+        o.s += row_sum<G>(listed);
     }
     const bool empty = o.m == -INFINITY && !(o.s != o.s);
     const float l2 = empty ? 0.f : log2_sum(o, c);
-    const float term = q == 0.f || e.at < 0 ? 0.f : q * (logq - logprob(e.x, o.m, l2, tp));
-    float loss = row_sum<G>(term);
+    float loss = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+        loss += q[i] == 0.f || e[i].at < 0 ? 0.f : q[i] * (logq[i] - logprob(e[i].x, o.m, l2, tp));
+    loss = row_sum<G>(loss);
     float B = empty ? 0.f : Q * fast_exp2(-(l2 + ms_slip(o.m, c)));
     if (TAIL) {
         // the mass the list leaves in 64 bits: a list that holds nearly everything leaves a small difference
-        const double left = 1.0 - group_sum_f64<G>(e.at >= 0 ? exp((double)e.t) : 0.0);
+        double mass = 0.0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) mass += e[i].at >= 0 ? exp((double)e[i].t) : 0.0;
+        const double left = 1.0 - group_sum_f64<G>(mass);
         const bool has_rest = rest.m > -INFINITY || rest.s != rest.s;
         const float qr = has_rest && left > 0.0 ? (float)left : 0.f;
         B = 0.f;
@@ -116,7 +160,7 @@ __device__ __forceinline__ void finish_row(i64 r, bool ok, int l, Online o, cons
             B = (Q + qr) * fast_exp2(to_all) - qr * fast_exp2(-(l2r + ms_slip(rest.m, c)));
         }
     }
-    const bool bad = group_allreduce_i32<G, OpMaxI>(e.bad ? 1 : 0) != 0;
+    bad = group_allreduce_i32<G, OpMaxI>(bad ? 1 : 0) != 0;
     if (bad && a.status) raise_flag(a.status, CWR_FLAG_BAD_LABEL);
     if (!ok || l != 0) return;
     a.loss[r] = bad ? __int_as_float(0x7fc00000) : loss / (float)(tp.inv * tp.inv);
@@ -124,7 +168,7 @@ __device__ __forceinline__ void finish_row(i64 r, bool ok, int l, Online o, cons
 }
 
 // G lanes per row (the row whole in registers), or one or NW waves per row that walk it in chunks.
-template <typename T, int G, int NW, bool TAIL, bool EDGE>
+template <typename T, int G, int E, int NW, bool TAIL, bool EDGE>
 __global__ __launch_bounds__(64 * (NW > 1 ? NW : kWavesPerBlock)) void k_distill(
     const T* __restrict__ x, i64 R, int V, i64 stride, const Temper tp, const DistillArgs a) {
     static_assert(NW == 1 || G == 64, "several waves share a row only as whole waves");
@@ -149,8 +193,9 @@ __global__ __launch_bounds__(64 * (NW > 1 ? NW : kWavesPerBlock)) void k_distill
     v4i next[NP];
     auto fetch = [&](int ch) { load_chunk<T, G, EDGE, false>(row, ch * CHUNK - off, l, V, next); };
     if (first_chunk < chunks) fetch(first_chunk);
-    const Entry e = load_entry<T>(row, rr, l, V, a.top, a.index, a.K);
-    bool first = e.at >= 0;
+    Entry e[E];
+    const bool bad = load_entries<T, G, E>(row, rr, l, V, a.top, a.index, a.K, e);
+    unsigned first = 0;
 
     Online o = {-INFINITY, 0.f, 0.f};
     for (int ch = first_chunk; ch < chunks; ch += NW) {
@@ -161,12 +206,15 @@ __global__ __launch_bounds__(64 * (NW > 1 ? NW : kWavesPerBlock)) void k_distill
         if (TAIL) {
             marks[w][lane] = 0;
             wave_sync();
-            const int place = e.at + off - ch * CHUNK;
-            if (e.at >= 0 && place >= 0 && place < CHUNK) {
-                const int pk = place / VEC;
-                const unsigned bit = 1u << ((pk / G) * VEC + (place & (VEC - 1)));
-                // of entries that name one index, the one that sets the mark counts
-                first = (atomicOr(&marks[w][g * G + (pk & (G - 1))], bit) & bit) == 0;
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const int place = e[i].at + off - ch * CHUNK;
+                if (e[i].at >= 0 && place >= 0 && place < CHUNK) {
+                    const int pk = place / VEC;
+                    const unsigned bit = 1u << ((pk / G) * VEC + (place & (VEC - 1)));
+                    // of entries that name one index, the one that sets the mark counts
+                    if ((atomicOr(&marks[w][g * G + (pk & (G - 1))], bit) & bit) == 0) first |= 1u << i;
+                }
             }
             wave_sync();
             const unsigned mine = marks[w][lane];
@@ -197,12 +245,13 @@ __global__ __launch_bounds__(64 * (NW > 1 ? NW : kWavesPerBlock)) void k_distill
             o.s += p.s;
         }
         if (TAIL) {  // the marks were set by several waves: the first of equal indices counts
-            first = e.at >= 0;
+            static_assert(NW == 1 || E == 1, "a wave has a lane for every entry");
+            first = e[0].at >= 0 ? 1u : 0u;
             for (int j = 0; j < a.K; ++j)
-                if (__builtin_amdgcn_readlane(e.at, j) == e.at && j < lane) first = false;
+                if (__builtin_amdgcn_readlane(e[0].at, j) == e[0].at && j < lane) first = 0;
         }
     }
-    finish_row<G, TAIL>(r, ok, l, o, e, first, tp, a);
+    finish_row<G, TAIL, E>(r, ok, l, o, e, first, bad, tp, a);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -272,7 +321,7 @@ constexpr int kUnset = 0x7fedcba9;  // a NaN no arithmetic here produces: not an
 // One wave per chunk of a row (G = 64) or per 64 / G whole rows.  Outside the list the gradient is one
 // exponential times a number of the row; each listed entry is worked out by one lane and put into a map
 // of the chunk in LDS, from where the pass over the chunk picks it up, so that every element is written once.
-template <typename T, int G, bool TAIL, bool EDGE>
+template <typename T, int G, int E, bool TAIL, bool EDGE>
 __global__ __launch_bounds__(kWavesPerBlock * 64) void k_distill_grad(
     const T* __restrict__ x, i64 R, int V, i64 stride, const Temper tp, const float* __restrict__ top,
     const int* __restrict__ index, int K, const float4* __restrict__ stat, const GradOut go, int chunks_per_row,
@@ -301,7 +350,8 @@ __global__ __launch_bounds__(kWavesPerBlock * 64) void k_distill_grad(
     const int e0 = ch * CHUNK - off;              // row element of map place 0
     v4i raw[NP];
     load_chunk<T, G, EDGE, false>(row, e0, l, V, raw);
-    const Entry e = load_entry<T>(row, r, l, V, top, index, K);
+    Entry e[E];
+    load_entries<T, G, E>(row, r, l, V, top, index, K, e);
     const float4 st = stat[r];
     float gt = go.p[r * go.stride] * go.scale / (float)tp.inv;
     int* map = map_[w] + g * CHUNK;
@@ -311,33 +361,49 @@ __global__ __launch_bounds__(kWavesPerBlock * 64) void k_distill_grad(
 #pragma unroll
         for (int j = 0; j < VEC; ++j) p[j] = kUnset;
     }
-    float q, logq, Q;
-    teacher<G, TAIL>(e, tp, q, logq, Q);
-    if (TAIL && (st.x > -INFINITY)) Q = fmaxf(Q, 1.f);  // with the tail's mass, where there is a tail
+    float q[E], logq[E], Q;
+    teacher<G, TAIL, E>(e, tp, q, logq, Q);
+    if (TAIL && st.x > -INFINITY) Q = fmaxf(Q, 1.f);  // with the tail's mass, where there is a tail
     const float c = tp.c;
     const Anchor ref = anchor(st.x, c);
     const bool poisoned = st.w == kPoisoned;
     const float B = poisoned ? 0.f : st.y * gt;
     wave_sync();
-    const int place = e.at - e0;
-    const bool here = e.at >= 0 && place >= 0 && place < CHUNK;
-    if (here) map[place] = lane;
+    int place[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        place[i] = e[i].at >= 0 && e[i].at >= e0 && e[i].at - e0 < CHUNK ? e[i].at - e0 : -1;
+        if (place[i] >= 0) map[place[i]] = l + i * G;
+    }
     wave_sync();
-    if (__ballot(here && map[place] != lane) != 0) {  // an index listed more than once: its shares add up, in order
-        float sum = 0.f;
-        for (int j = 0; j < K; ++j) {
-            const float qj = __shfl(q, g * G + j);
-            const int aj = __shfl(e.at, g * G + j);
-            sum += aj == e.at ? qj : 0.f;
+    bool twice = false;
+#pragma unroll
+    for (int i = 0; i < E; ++i) twice |= place[i] >= 0 && map[place[i]] != l + i * G;
+    if (__ballot(twice) != 0) {  // an index listed more than once: its shares add up, in the list's order
+        float sum[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) sum[i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < E; ++k)
+            for (int j = 0; j < G; ++j) {
+                const float qj = __shfl(q[k], g * G + j);
+                const int aj = __shfl(e[k].at, g * G + j);
+#pragma unroll
+                for (int i = 0; i < E; ++i) sum[i] += aj == e[i].at ? qj : 0.f;
+            }
+#pragma unroll
+        for (int i = 0; i < E; ++i) q[i] = sum[i];
+    }
+    wave_sync();
+    const bool empty = st.z == -INFINITY && st.w == st.w;
+    const Anchor anc = anchor(st.z, c);
+    const float total = st.w + ms_slip(st.z, c);
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+        if (place[i] >= 0) {
+            const float p = empty ? 0.f : fast_exp2(measure(e[i].x, anc, c) - total);
+            map[place[i]] = poisoned ? 0 : __float_as_int(gt * fmaf(p, Q, -q[i]));
         }
-        q = sum;
-    }
-    wave_sync();
-    if (here) {
-        const bool empty = st.z == -INFINITY && st.w == st.w;
-        const float p = empty ? 0.f : fast_exp2(measure(e.x, anchor(st.z, c), c) - (st.w + ms_slip(st.z, c)));
-        map[place] = poisoned ? 0 : __float_as_int(gt * fmaf(p, Q, -q));
-    }
     wave_sync();
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
@@ -369,30 +435,44 @@ __global__ __launch_bounds__(kWavesPerBlock * 64) void k_distill_grad(
 // ---------------------------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------------------------
+// Lanes per row: enough for the row, 16 elements each, and for its list, four entries each (a lane per entry
+// widened the group of a short row: 1022684 rows of 102 fp16 entries with lists of 34 took 1100 us, forward
+// and backward, with one row per wave).
+static int list_group(int span, int K) {
+    int G = 4;
+    while (G < 64 && (G * kLaneElems < span || 4 * G < K)) G *= 2;
+    return G;
+}
+
 template <typename T, bool TAIL, bool EDGE>
 static int distill_typed(const T* x, i64 R, int V, i64 stride, const Temper& tp, const DistillArgs& a,
                          hipStream_t stream) {
     const int span = V + (EDGE ? RowPacks<T>::VEC - 1 : 0);  // places a row can take on the pack grid
-    int G = 4;
-    while (G < 64 && (G * kLaneElems < span || G < a.K)) G *= 2;  // a lane for every list entry
-#define CWR_GROUP(GG)                                                                                               \
-    if (G == GG) {                                                                                                  \
+    const int G = list_group(span, a.K);
+#define CWR_GROUP_E(GG, EE)                                                                                         \
+    {                                                                                                               \
         const i64 waves = (R + 64 / GG - 1) / (64 / GG);                                                            \
         if (waves > 0x3fffffffLL * kWavesPerBlock) return CWR_ERR_TOO_LARGE;                                        \
-        CWR_LAUNCH((k_distill<T, GG, 1, TAIL, EDGE>), dim3(wave_blocks(waves)), dim3(kWavesPerBlock * 64), 0, stream, \
-                   x, R, V, stride, tp, a);                                                                         \
+        CWR_LAUNCH((k_distill<T, GG, EE, 1, TAIL, EDGE>), dim3(wave_blocks(waves)), dim3(kWavesPerBlock * 64), 0,   \
+                   stream, x, R, V, stride, tp, a);                                                                 \
         return check_launch();                                                                                      \
     }
+#define CWR_GROUP(GG)                                                                                               \
+    if (G == GG) {                                                                                                  \
+        if (a.K <= GG) CWR_GROUP_E(GG, 1)                                                                           \
+        CWR_GROUP_E(GG, 4)                                                                                          \
+    }
     CWR_GROUP(4) CWR_GROUP(8) CWR_GROUP(16) CWR_GROUP(32)
+#undef CWR_GROUP
     const i64 chunks = ((i64)span + 64 * kLaneElems - 1) / (64 * kLaneElems);
     const int NW = row_waves(R, chunks);
     if (R > 0x3fffffffLL) return CWR_ERR_TOO_LARGE;
-    if (NW == 1) { CWR_GROUP(64) }
-#undef CWR_GROUP
+    if (NW == 1) CWR_GROUP_E(64, 1)
+#undef CWR_GROUP_E
     if (NW == 16)
-        CWR_LAUNCH((k_distill<T, 64, 16, TAIL, EDGE>), dim3((unsigned)R), dim3(1024), 0, stream, x, R, V, stride, tp, a);
+        CWR_LAUNCH((k_distill<T, 64, 1, 16, TAIL, EDGE>), dim3((unsigned)R), dim3(1024), 0, stream, x, R, V, stride, tp, a);
     else
-        CWR_LAUNCH((k_distill<T, 64, 4, TAIL, EDGE>), dim3((unsigned)R), dim3(256), 0, stream, x, R, V, stride, tp, a);
+        CWR_LAUNCH((k_distill<T, 64, 1, 4, TAIL, EDGE>), dim3((unsigned)R), dim3(256), 0, stream, x, R, V, stride, tp, a);
     return check_launch();
 }
 
@@ -400,19 +480,26 @@ template <typename T, bool TAIL, bool EDGE>
 static int distill_grad_typed(const T* x, i64 R, int V, i64 stride, const Temper& tp, const RowDistill& s, const GradOut& go,
                               T* dx, hipStream_t stream) {
     const int span = V + (EDGE ? RowPacks<T>::VEC - 1 : 0);
-    int G = 4;
-    while (G < 64 && (G * kLaneElems < span || G < s.K)) G *= 2;
+    const int G = list_group(span, (int)s.K);
     const i64 chunks = G < 64 ? 1 : ((i64)span + 64 * kLaneElems - 1) / (64 * kLaneElems);
     const i64 waves = G < 64 ? (R + 64 / G - 1) / (64 / G) : R * chunks;
     if (waves > 0x3fffffffLL * kWavesPerBlock) return CWR_ERR_TOO_LARGE;
-#define CWR_GROUP(GG)                                                                                                  \
-    if (G == GG)                                                                                                       \
-        CWR_LAUNCH((k_distill_grad<T, GG, TAIL, EDGE>), dim3(wave_blocks(waves)), dim3(kWavesPerBlock * 64), 0, stream, \
-                   x, R, V, stride, tp, s.top, s.index, (int)s.K, reinterpret_cast<const float4*>(s.stat), go,          \
-                   (int)chunks, dx);
-    CWR_GROUP(4) CWR_GROUP(8) CWR_GROUP(16) CWR_GROUP(32) CWR_GROUP(64)
+#define CWR_GROUP_E(GG, EE)                                                                                              \
+    {                                                                                                                    \
+        CWR_LAUNCH((k_distill_grad<T, GG, EE, TAIL, EDGE>), dim3(wave_blocks(waves)), dim3(kWavesPerBlock * 64), 0,      \
+                   stream, x, R, V, stride, tp, s.top, s.index, (int)s.K, reinterpret_cast<const float4*>(s.stat), go,   \
+                   (int)chunks, dx);                                                                                     \
+        return check_launch();                                                                                           \
+    }
+#define CWR_GROUP(GG)                                                                                                    \
+    if (G == GG) {                                                                                                       \
+        if (s.K <= GG) CWR_GROUP_E(GG, 1)                                                                                \
+        CWR_GROUP_E(GG, 4)                                                                                               \
+    }
+    CWR_GROUP(4) CWR_GROUP(8) CWR_GROUP(16) CWR_GROUP(32)
+    CWR_GROUP_E(64, 1)
 #undef CWR_GROUP
-    return check_launch();
+#undef CWR_GROUP_E
 }
 
 template <typename T>
