@@ -582,7 +582,7 @@ static int check_rows(const void* x, int dtype, int64_t R, int64_t V, int64_t x_
     if (R < 0 || V < 1 || x_stride < 0 || K < 0) return CWR_ERR_SHAPE;
     if (V >= 1 << 28) return CWR_ERR_TOO_LARGE;
     if (K > CWR_MAX_ROW_TOKENS) return CWR_ERR_TOO_LARGE;
-    if (!(temperature > 0.0) || !(temperature <= 1e30) || temperature < 1e-30) return CWR_ERR_SHAPE;
+    if (!(temperature >= 1e-6 && temperature <= 1e6)) return CWR_ERR_SHAPE;
     if (R > 0 && !x) return CWR_ERR_NULL;
     if (misaligned(x, elem_size(dtype))) return CWR_ERR_ALIGN;
     return CWR_OK;

@@ -277,6 +277,9 @@ __device__ __forceinline__ float logprob(float x, float m, float l2, const Tempe
 // ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
+// Waves of 64 work-items a launch can hold: the runtime counts work-items in 32 bits.
+constexpr i64 kMaxWaves = ((i64)1 << 26) - 64;
+
 inline unsigned wave_blocks(i64 waves) {  // whole workgroups, a multiple of the XCDs
     return (unsigned)(((waves + kWavesPerBlock - 1) / kWavesPerBlock + 7) & ~(i64)7);
 }

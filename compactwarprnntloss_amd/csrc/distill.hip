@@ -452,7 +452,7 @@ static int distill_typed(const T* x, i64 R, int V, i64 stride, const Temper& tp,
 #define CWR_GROUP_E(GG, EE)                                                                                         \
     {                                                                                                               \
         const i64 waves = (R + 64 / GG - 1) / (64 / GG);                                                            \
-        if (waves > 0x3fffffffLL * kWavesPerBlock) return CWR_ERR_TOO_LARGE;                                        \
+        if (waves > kMaxWaves) return CWR_ERR_TOO_LARGE;                                        \
         CWR_LAUNCH((k_distill<T, GG, EE, 1, TAIL, EDGE>), dim3(wave_blocks(waves)), dim3(kWavesPerBlock * 64), 0,   \
                    stream, x, R, V, stride, tp, a);                                                                 \
         return check_launch();                                                                                      \
@@ -466,7 +466,7 @@ static int distill_typed(const T* x, i64 R, int V, i64 stride, const Temper& tp,
 #undef CWR_GROUP
     const i64 chunks = ((i64)span + 64 * kLaneElems - 1) / (64 * kLaneElems);
     const int NW = row_waves(R, chunks);
-    if (R > 0x3fffffffLL) return CWR_ERR_TOO_LARGE;
+    if (R > kMaxWaves) return CWR_ERR_TOO_LARGE;
     if (NW == 1) CWR_GROUP_E(64, 1)
 #undef CWR_GROUP_E
     if (NW == 16)
@@ -483,7 +483,7 @@ static int distill_grad_typed(const T* x, i64 R, int V, i64 stride, const Temper
     const int G = list_group(span, (int)s.K);
     const i64 chunks = G < 64 ? 1 : ((i64)span + 64 * kLaneElems - 1) / (64 * kLaneElems);
     const i64 waves = G < 64 ? (R + 64 / G - 1) / (64 / G) : R * chunks;
-    if (waves > 0x3fffffffLL * kWavesPerBlock) return CWR_ERR_TOO_LARGE;
+    if (waves > kMaxWaves) return CWR_ERR_TOO_LARGE;
 #define CWR_GROUP_E(GG, EE)                                                                                              \
     {                                                                                                                    \
         CWR_LAUNCH((k_distill_grad<T, GG, EE, TAIL, EDGE>), dim3(wave_blocks(waves)), dim3(kWavesPerBlock * 64), 0,      \

@@ -559,7 +559,7 @@ static int scores_typed(const T* x, i64 R, int V, i64 stride, const Temper& tp, 
 #define CWR_GROUP(GG)                                                                                              \
     if (G == GG) {                                                                                                 \
         const i64 waves = (R + 64 / GG - 1) / (64 / GG);                                                           \
-        if (waves > 0x3fffffffLL * kWavesPerBlock) return CWR_ERR_TOO_LARGE;                                       \
+        if (waves > kMaxWaves) return CWR_ERR_TOO_LARGE;                                       \
         CWR_LAUNCH((k_scores_group<T, GG, EDGE>), dim3(wave_blocks(waves)), dim3(kWavesPerBlock * 64), 0, stream, x, \
                    R, V, stride, tp, a);                                                                           \
         return check_launch();                                                                                     \
@@ -568,7 +568,7 @@ static int scores_typed(const T* x, i64 R, int V, i64 stride, const Temper& tp, 
 #undef CWR_GROUP
     const i64 chunks = ((i64)span + 64 * kLaneElems - 1) / (64 * kLaneElems);
     const int NW = row_waves(R, chunks);
-    if (R > 0x3fffffffLL) return CWR_ERR_TOO_LARGE;
+    if (R > kMaxWaves) return CWR_ERR_TOO_LARGE;
     if (NW == 16)
         CWR_LAUNCH((k_scores_wave<T, 16, EDGE>), dim3((unsigned)R), dim3(1024), 0, stream, x, R, V, stride, tp, a);
     else if (NW == 4)
@@ -588,7 +588,7 @@ static int scores_grad_typed(const T* x, i64 R, int V, i64 stride, const Temper&
     while (G < 64 && (G * kLaneElems < span || 2 * G < n)) G *= 2;  // two entries a lane at most
     const i64 chunks = G < 64 ? 1 : ((i64)span + 64 * kLaneElems - 1) / (64 * kLaneElems);
     const i64 waves = G < 64 ? (R + 64 / G - 1) / (64 / G) : R * chunks;
-    if (waves > 0x3fffffffLL * kWavesPerBlock) return CWR_ERR_TOO_LARGE;
+    if (waves > kMaxWaves) return CWR_ERR_TOO_LARGE;
 #define CWR_GROUP(GG)                                                                                               \
     if (G == GG)                                                                                                    \
         CWR_LAUNCH((k_scores_grad<T, GG, EDGE>), dim3(wave_blocks(waves)), dim3(kWavesPerBlock * 64), 0, stream, x, \

@@ -62,8 +62,8 @@ def _check_rows(x: torch.Tensor, temperature: float):
         raise RuntimeError("x must have at least one entry per row")
     if x.size(1) > 1 and x.stride(1) != 1:
         raise RuntimeError("the entries of a row of x must be adjacent (rows may be any distance apart)")
-    if not (1e-30 <= temperature <= 1e30):
-        raise RuntimeError("temperature must be positive and finite")
+    if not (1e-6 <= temperature <= 1e6):
+        raise RuntimeError("temperature must lie between 1e-6 and 1e6")
 
 
 def _check_tokens(tokens: Optional[torch.Tensor], R: int, device) -> int:
@@ -320,7 +320,7 @@ def distill_loss(x: torch.Tensor, top_logits: torch.Tensor, top_index: torch.Ten
 def lattice_tokens(lx: torch.Tensor, y: torch.Tensor, ly: torch.Tensor, total_rows: int, V: int,
                    blank: int = 0) -> torch.Tensor:
     """(total_rows, 2) int32: the blank and the label of every compact row, -1 where a row has no label (the
-    last label position of a sequence) or belongs to no sequence: the `tokens` under which token_logprobs
+    last label position of a sequence, or a label outside [0, V)) or belongs to no sequence: the `tokens` under which token_logprobs
     returns the pair of log-probabilities the loss walks on.
 
     lx, ly, y as for transducer_loss; total_rows = sum_i lx_i*(ly_i+1)."""

@@ -346,14 +346,15 @@ int cwr_joint_backward(const void* h, const void* w, const float* bias, int dtyp
  * (test/test.py:19-20).  The compact rows of a lattice are scored with tokens (blank, label).
  *   x            (R, V) of any cwr_dtype (64-bit entries are rounded to fp32 when read, as everywhere in
  *                this library), row r at x + r * x_stride, entries of a row adjacent; x_stride >= 0; V < 2^28
- *   tokens       (R, M) int32, M <= 64;  K <= 64, K <= V;  temperature > 0 and finite
+ *   tokens       (R, M) int32, M <= 64;  K <= 64, K <= V;  1e-6 <= temperature <= 1e6
  *   stat         (R, 4) fp32, 16-byte aligned, for cwr_token_logprobs_backward: row maximum, log2 of the scaled
  *                sum, entropy, 0;  NULL: not kept
  *   logprobs     (R, M) fp32, NULL only if M = 0;  entropy, lse (R) fp32, each may be NULL
  *   top_logprobs (R, K) fp32 and top_index (R, K) int32, NULL only if K = 0
  *   status       4 x int32 the caller has zeroed, or NULL
  * A row of nothing but -inf: lse = -inf, log-probabilities -inf, entropy 0, gradient 0.  A row with NaN or
- * +inf in it: everything but top_index is NaN. */
+ * +inf in it: everything but top_index is NaN.  CWR_ERR_TOO_LARGE for more rows than one launch counts
+ * (2^26 of more than 512 entries, or as many chunks of 1024 entries in the backward pass). */
 #define CWR_MAX_ROW_TOKENS 64
 int cwr_token_logprobs(const void* x, int dtype, int64_t R, int64_t V, int64_t x_stride, const int32_t* tokens,
                        int64_t M, int64_t K, double temperature, float* stat, float* logprobs, float* entropy,

@@ -200,3 +200,34 @@ def test_gradient_against_differences():
                     d = (f(x + e).double() - f(x - e).double()) / (2 * h)
                 # third derivative of T^2 KL in x: below 1 / T; the sum's own error, 1e-6 a side
                 assert abs(float(d) - float(dx[i, v])) <= h * h + 4e-6 / h
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V", [40, 1024, 5000])
+def test_rows_masked_with_the_lowest_value(V, dtype):
+    """Entries at the type's lowest value are masked entries; a row of nothing else is uniform."""
+    x, top, idx, gen = make(6, V, 3, dtype, False, 1.0, absent=0.0, seed=V)
+    low = torch.finfo(dtype).min
+    keep = torch.zeros((6, V), dtype=torch.bool, device=DEV).scatter_(1, idx.long(), True)
+    x[1:4] = torch.where(keep[1:4], x[1:4], low)
+    check(x[:4], top[:4], idx[:4], 1.0, False, gen, dtype)
+    x[4] = low
+    x.requires_grad_(True)
+    loss = pkg.distill_loss(x, top, idx, reduction="none")
+    q = torch.softmax(top[4].double(), 0)
+    want = float((q * (q.log() + math.log(V))).sum())
+    assert abs(float(loss[4]) - want) <= EPS32 * 100 * (1 + want)
+    dx, = torch.autograd.grad(loss[4], x)
+    ref = torch.full((V,), 1.0 / V, dtype=torch.float64, device=DEV).scatter_add_(0, idx[4].long(), -q)
+    assert float((dx[4].double() - ref).abs().max()) <= half_step(dtype) + EPS32 * 100
+    tailed = pkg.distill_loss(x, top - 20.0, idx, tail=True, reduction="none")
+    dt, = torch.autograd.grad(tailed.sum(), x)
+    assert torch.isfinite(dt[4]).all() and torch.isfinite(tailed[4])
+
+
+def test_a_list_longer_than_the_vocabulary():
+    x, top, idx, gen = make(50, 5, 5, torch.float32, True, 1.0, absent=0.0)
+    long_top = torch.cat([top, top], 1) - math.log(2.0)
+    long_idx = torch.cat([idx, idx], 1)
+    check(x, long_top, long_idx, 1.0, True, gen, torch.float32)
+    check(x, long_top, long_idx, 1.0, False, gen, torch.float32)

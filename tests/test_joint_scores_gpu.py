@@ -30,7 +30,10 @@ def grid_problem(R, V, H, dtype, seed=0, bias="same"):
 
 SHAPES = [(1, 32, 32, 1), (1, 1024, 512, 4), (5, 41, 64, 3), (8, 1000, 640, 8), (32, 33, 96, 33), (33, 1027, 128, 16),
           (64, 50, 1024, 8), (65, 4096, 640, 8), (512, 1024, 320, 4), (1000, 130, 160, 5), (1025, 257, 128, 4),
-          (1100, 5000, 512, 8), (2000, 1024, 1024, 4), (3000, 129, 704, 2), (1500, 300, 1056, 3), (5000, 41, 256, 8)]
+          (1100, 5000, 512, 8), (2000, 1024, 1024, 4), (3000, 129, 704, 2), (1500, 300, 1056, 3), (5000, 41, 256, 8),
+          # large products: the walks with resident rows (their three kinds of shapes) and with streamed rows
+          (3300, 4100, 512, 4), (12500, 1001, 704, 4), (12300, 1024, 1024, 2), (12101, 1003, 640, 8), (48001, 257, 192, 3),
+          (13000, 1000, 96, 3), (12100, 1027, 1056, 4)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
