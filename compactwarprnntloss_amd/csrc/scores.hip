@@ -242,6 +242,15 @@ __device__ __forceinline__ void rank_append(Ranking& q, float f, int e, bool in)
     q.n += __popcll(takers);
 }
 
+// Cuts the list back to its best K and raises the bound to the last of them.
+__device__ __forceinline__ void rank_tighten(Ranking& q, int K) {
+    q.n = list_compress(q.list, q.n, K);
+    if (q.n == K) {
+        q.bound = q.list[K - 1];
+        q.floor_ = key_value(q.bound);
+    }
+}
+
 // v[s] for a slot that differs between the lanes: selects of values (a choice between elements of the
 // array itself would put the array into memory)
 __device__ __forceinline__ float pick(bool second, float x, float y) { return second ? y : x; }
@@ -270,13 +279,7 @@ __device__ __forceinline__ void rank_chunk(Ranking& q, const float (&v)[kLaneEle
         const u64 some = __ballot(reach != 0);
         if (some == 0) break;
         // many equal or many rising values: the list is cut back, and the bound raised, as often as it fills up
-        if (q.n + __popcll(some) > kListCap) {
-            q.n = list_compress(q.list, q.n, K);
-            if (q.n == K) {
-                q.bound = q.list[K - 1];
-                q.floor_ = key_value(q.bound);
-            }
-        }
+        if (q.n + __popcll(some) > kListCap) rank_tighten(q, K);
         const unsigned s = (unsigned)(__ffs((int)reach) - 1) & 15u;  // (none left: any)
         const float f = pick16(v, s);
         const int e = e0 + (int)((s / VEC) * 64 * VEC + (s & (VEC - 1)));
@@ -334,6 +337,9 @@ __global__ __launch_bounds__(64 * (NW > 1 ? NW : kWavesPerBlock), sizeof(T) == 2
             q.bound = (u64)((unsigned)lo ^ 0x80000000u) << 32;  // below every key of that value
         }
         rank_chunk<VEC>(q, v, best, ch * CHUNK + lane * VEC - off, V, a.K);
+        // before more chunks: a bound as tight as the list allows, or every chunk hands in as many as the first
+        // (2048 rows of 50257 bf16 entries, K = 32: 79 us without)
+        if (ch + NW < chunks && (ch == first || q.n > a.K + a.K / 2 + 8)) rank_tighten(q, a.K);
     }
 
     // the lanes' sums, then the waves'
