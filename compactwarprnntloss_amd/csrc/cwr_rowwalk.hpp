@@ -269,9 +269,20 @@ __device__ __forceinline__ float log2_sum(const Online& o, float c) { return log
 // ln p of the logit x in a row with maximum m and log2 sum l2.  The difference x - m is exact in 64 bits and
 // the logarithm of the sum is small in a peaked row: the result keeps its absolute accuracy however
 // large the logits are.  A row of nothing but -inf gives -inf.
-__device__ __forceinline__ float logprob(float x, float m, float l2, const Temper& tp) {
+__device__ __forceinline__ double logprob_f64(float x, float m, double l2, const Temper& tp) {
     if (x == -INFINITY && !(l2 != l2)) return -INFINITY;
-    return (float)(((double)x - (double)m) * tp.inv - (double)l2 * 0.6931471805599453);
+    return ((double)x - (double)m) * tp.inv - l2 * 0.6931471805599453;
+}
+__device__ __forceinline__ float logprob(float x, float m, float l2, const Temper& tp) {
+    return (float)logprob_f64(x, m, (double)l2, tp);
+}
+
+// log2 of a number >= 0: exact to about 1e-7, and next to 1 to as much of the result itself.  The exponent stands
+// apart from the logarithm of the mantissa (as one fp32 number the logarithm of 1000 is off by 5e-7).
+__device__ __forceinline__ double log2_f64(float s) {
+    if (fabsf(s - 1.f) < 0.015625f) return (double)log2_of_sum(s);  // its series, on both sides of 1
+    const float f = 2.f * __builtin_amdgcn_frexp_mantf(s);          // [1, 2)
+    return (double)(__builtin_amdgcn_frexp_expf(s) - 1) + (double)log2_of_sum(f);
 }
 
 // ---------------------------------------------------------------------------------------------

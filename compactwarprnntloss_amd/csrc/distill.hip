@@ -155,11 +155,14 @@ __device__ __forceinline__ void finish_row(i64 r, bool ok, int l, Online o, cons
         o.s += row_sum<G>(listed);
     }
     const bool empty = o.m == -INFINITY && !(o.s != o.s);
-    const float l2 = empty ? 0.f : log2_sum(o, c);
+    // Where teacher and student nearly agree the loss is the small rest of differences of logarithms: those are
+    // taken in 64 bits (an error of the row's sum itself cancels, the shares being nearly those of the teacher).
+    const double l2d = empty ? 0.0 : log2_f64(o.s) - (double)ms_slip(o.m, c);
+    const float l2 = (float)l2d;
     float loss = 0.f;
 #pragma unroll
     for (int i = 0; i < E; ++i)
-        loss += q[i] == 0.f || e[i].at < 0 ? 0.f : q[i] * (logq[i] - logprob(e[i].x, o.m, l2, tp));
+        loss += q[i] == 0.f || e[i].at < 0 ? 0.f : q[i] * (float)((double)logq[i] - logprob_f64(e[i].x, o.m, l2d, tp));
     loss = row_sum<G>(loss);
     float B = empty ? 0.f : Q * fast_exp2(-(l2 + ms_slip(o.m, c)));
     if (TAIL) {
@@ -172,10 +175,12 @@ __device__ __forceinline__ void finish_row(i64 r, bool ok, int l, Online o, cons
         const float qr = has_rest && left > 0.0 ? (float)left : 0.f;
         B = 0.f;
         if (has_rest) {
-            const float l2r = log2_sum(rest, c);
-            const float logpr = (float)(((double)rest.m - (double)o.m) * tp.inv +
-                                        ((double)l2r - (double)l2) * 0.6931471805599453);
-            if (qr > 0.f) loss += qr * (kLn2 * fast_log2(qr) - logpr);
+            const double l2rd = log2_f64(rest.s) - (double)ms_slip(rest.m, c);
+            const float l2r = (float)l2rd;
+            if (qr > 0.f) {
+                const double logpr = ((double)rest.m - (double)o.m) * tp.inv + (l2rd - l2d) * 0.6931471805599453;
+                loss += qr * (float)(log2_f64(qr) * 0.6931471805599453 - logpr);
+            }
             const float to_all = anchor_shift(rest.m, o.m, c) - (l2 + ms_slip(o.m, c));
             B = (Q + qr) * fast_exp2(to_all) - qr * fast_exp2(-(l2r + ms_slip(rest.m, c)));
         }

@@ -231,3 +231,38 @@ def test_a_list_longer_than_the_vocabulary():
     long_idx = torch.cat([idx, idx], 1)
     check(x, long_top, long_idx, 1.0, True, gen, torch.float32)
     check(x, long_top, long_idx, 1.0, False, gen, torch.float32)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,K", [(100003, 4), (70001, 1)])
+def test_a_student_that_agrees_with_its_teacher(V, K, dtype):
+    """The loss is far below the logarithms it is a difference of."""
+    gen = torch.Generator(device=DEV).manual_seed(V)
+    x = (torch.randn((64, V), device=DEV, generator=gen) * 0.25).to(dtype)
+    t = x.double() + 0.02 * torch.randn((64, V), device=DEV, generator=gen).double()
+    T = 2.0
+    top, idx = torch.log_softmax(t / T, 1).topk(K, dim=1)
+    top, idx = top.float(), idx.to(torch.int32)
+    loss = pkg.distill_loss(x, top, idx, temperature=T, tail=True, reduction="none")
+    want = distill_ref(x, top, idx, T, True)[0]
+    # The listed mass is below 1e-3 and the row's sum enters by p_r - q_r only, so what is left are, for q_r near
+    # 1: two logarithms of a mantissa in [1, 2) (1e-7 or 2 half steps each, log 2 of it after the change of base),
+    # the move of the rest's sum to the maximum of all (2^d to 2, its product and the addition of the list 1
+    # each), q_r as a number of 32 bits 1, and the sum of the terms 1: below 9 half steps, times T^2.
+    assert float((loss.double() - want).abs().max()) <= 9 * EPS32 * T * T
+    # (one fp32 number for a logarithm near 17 would be off by 16 half steps alone)
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("V", [32, 1024, 6000])
+def test_a_student_with_nothing(V, tail):
+    x, top, idx, _ = make(3, V, 2, torch.float32, tail, 1.0, absent=0.0)
+    x[1] = -math.inf
+    want = torch.zeros(V, device=DEV).double()
+    want[idx[1].long()] = -(top[1].double().exp() if tail else torch.softmax(top[1].double(), 0))
+    x.requires_grad_(True)
+    loss = pkg.distill_loss(x, top, idx, tail=tail, reduction="none")
+    assert float(loss[1]) == math.inf and torch.isfinite(loss[0]) and torch.isfinite(loss[2])
+    dx, = torch.autograd.grad(loss, x, torch.ones_like(loss))
+    # p = 0 everywhere leaves -q; q to its exponential, its sum and their quotient
+    assert float((dx[1].double() - want).abs().max()) <= 16 * EPS32
