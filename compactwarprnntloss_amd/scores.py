@@ -288,6 +288,8 @@ def distill_loss(x: torch.Tensor, top_logits: torch.Tensor, top_index: torch.Ten
     validate    read the status word back (one synchronisation) and raise when an index lies outside
                 [-1, V); without it the loss of such a row is NaN and its gradient 0
 
+    A listed entry that the student has at -inf makes the loss infinite; the gradient takes its p as 0.
+
     Differentiable in x; the teacher gets no gradient."""
     assert reduction in ["mean", "sum", "none"] or reduction is None
     temperature = float(temperature)
