@@ -177,14 +177,16 @@ struct Online {
     float m, s, u;
 };
 
-// What elements are measured against: t = fma(x - sub, c, -ms).  Normally sub = 0 and ms = m c rounded to
-// fp32: one fma per element, and what the rounding loses is the same for the whole row and comes back
-// exactly from an fma (ms_slip).  Where m c is out of all proportion (rows masked with the lowest
-// value of their type) that product would overflow, and m is subtracted first.
+// What elements are measured against: t = fma(x - sub, c, -ms).  Normally sub = 0 and ms = m c rounded to fp32: one
+// fma per element, and what the rounding loses is the same for the whole row and comes back exactly from an
+// fma (ms_slip).  It also stands in every exponent, as a factor 2^slip of the row's sum, so it has to stay
+// a small fraction of a bit: from |m c| = 2^16 on, where it could be more than 2^-9, m is subtracted first and the
+// sum's largest term is 1.  (Rows and chunks masked with a finite constant, logits far from zero, small
+// temperatures.)  A sum is then never below 1 - 2^-9, where the series of log2_of_sum is as exact as above 1.
 struct Anchor {
     float sub, ms;
 };
-__device__ __forceinline__ bool far_off(float m, float c) { return !(fabsf(m * c) < 0x1p100f); }  // NaN, inf too
+__device__ __forceinline__ bool far_off(float m, float c) { return !(fabsf(m * c) < 0x1p16f); }  // NaN, inf too
 __device__ __forceinline__ Anchor anchor(float m, float c) {
     Anchor a = {0.f, m * c};
     if (far_off(m, c)) {
@@ -198,10 +200,18 @@ __device__ __forceinline__ float measure(float x, const Anchor& a, float c) { re
 __device__ __forceinline__ float ms_slip(float m, float c) {  // m c - ms
     return far_off(m, c) ? 0.f : fmaf(m, c, -(m * c));
 }
-// how far, in bits, what is measured against `from` lies below what is measured against `to` >= from
+// How far, in bits, what is measured against `from` lies below what is measured against `to` >= from: the difference
+// of ms where there is one, of m c where it was subtracted exactly.  Products as they are rounded in `anchor`:
+// contracted into an fma the difference would be off by a slip.
 __device__ __forceinline__ float anchor_shift(float from, float to, float c) {
+#pragma clang fp contract(off)
     if (from == to) return 0.f;
-    return far_off(from, c) || far_off(to, c) ? -INFINITY : from * c - to * c;
+    const bool far_from = far_off(from, c), far_to = far_off(to, c);
+    const float mf = from * c, mt = to * c;
+    if (!far_from && !far_to) return mf - mt;
+    const double a = far_from ? (double)from * (double)c : (double)mf;
+    const double b = far_to ? (double)to * (double)c : (double)mt;
+    return (float)(a - b);  // -inf: nothing was there, or too far to matter
 }
 
 constexpr float kTFloor = -1024.f;  // 2^t is 0 far above it; keeps 0 * t finite where x is -inf
