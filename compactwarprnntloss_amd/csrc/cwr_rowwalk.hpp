@@ -206,12 +206,13 @@ __device__ __forceinline__ float ms_slip(float m, float c) {  // m c - ms
 __device__ __forceinline__ float anchor_shift(float from, float to, float c) {
 #pragma clang fp contract(off)
     if (from == to) return 0.f;
+    if (from == -INFINITY) return -INFINITY;  // nothing was there
     const bool far_from = far_off(from, c), far_to = far_off(to, c);
     const float mf = from * c, mt = to * c;
     if (!far_from && !far_to) return mf - mt;
     const double a = far_from ? (double)from * (double)c : (double)mf;
     const double b = far_to ? (double)to * (double)c : (double)mt;
-    return (float)(a - b);  // -inf: nothing was there, or too far to matter
+    return (float)(a - b);
 }
 
 constexpr float kTFloor = -1024.f;  // 2^t is 0 far above it; keeps 0 * t finite where x is -inf
