@@ -64,6 +64,53 @@ def stale_scc_reads(asm_text: str):
     return found
 
 
+# A vector instruction may read a scalar register (a condition mask, a carry) that another vector instruction wrote
+# only two wait states later.  The compiler keeps that distance between the instructions it chooses itself,
+# but it does not look into inline assembly: the device assembly is checked as a whole.
+_VALU_TWO_RESULTS = re.compile(r"v_(add_co|sub_co|subrev_co|addc|subb|subbrev|div_scale|mad_u64|mad_i64)")
+
+
+def _scalar_registers(operand: str):
+    operand = operand.strip().split(" ")[0]
+    if operand in ("vcc", "vcc_lo", "vcc_hi"):
+        return {"vcc_lo", "vcc_hi"} if operand == "vcc" else {operand}
+    m = re.fullmatch(r"s(\d+)|s\[(\d+):(\d+)\]", operand)
+    if not m:
+        return set()
+    lo, hi = (m.group(1), m.group(1)) if m.group(1) else (m.group(2), m.group(3))
+    return {f"s{i}" for i in range(int(lo), int(hi) + 1)}
+
+
+def early_scalar_reads(asm_text: str):
+    """Lines (1-based number, text) of the device assembly whose vector instruction reads a scalar register that a
+    vector instruction wrote fewer than two wait states before."""
+    found = []
+    recent = []  # (wait states since, registers a vector instruction wrote)
+    for i, line in enumerate(asm_text.split("\n")):
+        text = line.split(";")[0].split("//")[0].strip()
+        if text.endswith(":"):
+            recent = []
+            continue
+        if not text or text.startswith("."):
+            continue
+        op, _, rest = text.partition(" ")
+        operands = rest.split(",")
+        states = int(operands[0], 0) + 1 if op == "s_nop" else 1
+        written = set()
+        if op.startswith("v_"):
+            results = 2 if _VALU_TWO_RESULTS.match(op) else 1
+            read = set().union(*map(_scalar_registers, operands[results:]))
+            if op.startswith("v_div_fmas"):
+                read |= {"vcc_lo", "vcc_hi"}
+            if any(age < 2 and regs & read for age, regs in recent):
+                found.append((i + 1, text))
+            written = set().union(*map(_scalar_registers, operands[:results]))
+        recent = [(age + states, regs) for age, regs in recent if age + states < 2]
+        if written:
+            recent.append((0, written))
+    return found
+
+
 def _hipcc() -> str:
     exe = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
     if not os.path.exists(exe):
@@ -91,9 +138,13 @@ def build(verbose: bool = True) -> str:
             print(err, file=sys.stderr)
         asm = os.path.join(objdir, src.replace(".hip", f"-hip-amdgcn-amd-amdhsa-{ARCH}.s"))
         with open(asm) as f:
-            bad = stale_scc_reads(f.read())
+            asm_text = f.read()
+        bad = stale_scc_reads(asm_text)
         if bad:
             raise RuntimeError(f"{src}: scalar condition code read without a matching compare at {asm}: {bad[:5]}")
+        bad = early_scalar_reads(asm_text)
+        if bad:
+            raise RuntimeError(f"{src}: scalar register read too soon after a vector write at {asm}: {bad[:5]}")
         return obj
 
     with ThreadPoolExecutor(max_workers=min(9, len(SOURCES))) as ex:

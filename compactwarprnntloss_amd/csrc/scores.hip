@@ -263,18 +263,28 @@ __device__ __forceinline__ float pick16(const float (&v)[kLaneElems], unsigned s
     return pick(s8, pick(s4, b0, b1), pick(s4, b2, b3));
 }
 
+// Bit s: v[s] >= bound (and, above the largest finite number, more).  The sign of v - bound is shifted in, two
+// instructions a value and no scalar register between them: a vector instruction may read one that another vector
+// instruction wrote (a compare's result as a carry) only two wait states later.  The bound is the wave's and its
+// exceptions are settled on the scalar unit: zero is taken as -0, so that -0 - bound is +0; everything reaches
+// -inf, and +inf is let in by the largest finite number (the difference of two infinities has no sign).
+__device__ __forceinline__ unsigned reach_mask(const float (&v)[kLaneElems], float bound) {
+    constexpr unsigned all = (1u << kLaneElems) - 1;
+    const int bits = __builtin_amdgcn_readfirstlane(__float_as_int(bound));
+    if (bits == (int)0xff800000) return all;
+    const float f = __int_as_float(bits == 0 ? (int)0x80000000 : bits == 0x7f800000 ? 0x7f7fffff : bits);
+    unsigned below = 0;
+#pragma unroll
+    for (int s = kLaneElems - 1; s >= 0; --s) below = __builtin_amdgcn_alignbit(below, (unsigned)__float_as_int(v[s] - f), 31);
+    return ~below & all;
+}
+
 template <int VEC>
 __device__ __forceinline__ void rank_chunk(Ranking& q, const float (&v)[kLaneElems], float best, int e0, int V, int K) {
     if (__ballot(best >= q.floor_) == 0) return;
     // every lane notes which of its values reach the bound; all lanes then hand in one of them at a time
     // (about one lane in eight has any, hardly one has two)
-    unsigned reach = 0;
-#pragma unroll
-    for (int s = kLaneElems - 1; s >= 0; --s)  // a compare, and its result shifted in as a carry
-        asm("v_cmp_le_f32 vcc, %1, %2\n\tv_addc_co_u32 %0, vcc, %0, %0, vcc"
-            : "+v"(reach)
-            : "v"(q.floor_), "v"(v[s])
-            : "vcc");
+    unsigned reach = reach_mask(v, q.floor_);
     for (;;) {
         const u64 some = __ballot(reach != 0);
         if (some == 0) break;
