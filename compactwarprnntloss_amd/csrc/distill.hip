@@ -83,8 +83,8 @@ __device__ __forceinline__ void teacher(const Entry (&e)[E], const Temper& tp, f
     float mt = -INFINITY;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-        logq[i] = (float)((double)e[i].t * tp.inv);
-        mt = fmaxf(mt, logq[i]);
+        logq[i] = e[i].t;
+        mt = fmaxf(mt, e[i].t);
     }
     mt = row_max<G>(mt);
     if (mt == -INFINITY) {  // an empty list, or one of -inf only (or NaN)
@@ -96,9 +96,11 @@ __device__ __forceinline__ void teacher(const Entry (&e)[E], const Temper& tp, f
         Q = row_sum<G>(sum);
         return;
     }
+    // the difference first, in 64 bits: t / T as one fp32 number is off by half a step of its own, which for values far
+    // from zero or a small T is no small part of the difference
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-        logq[i] -= mt;
+        logq[i] = (float)(((double)e[i].t - (double)mt) * tp.inv);
         q[i] = fast_exp2(logq[i] * kLog2e);
         sum += q[i];
     }
