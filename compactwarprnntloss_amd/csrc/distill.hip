@@ -134,7 +134,9 @@ __device__ __forceinline__ double exp_f64(float t) {
     return t != t ? (double)t : ldexp(p, (int)n);
 }
 
-constexpr float kPoisoned = INFINITY;  // in place of a row's log2 sum: an index outside the vocabulary was met
+// In place of a row's log2 sum: nothing is to be learned from this row, its gradient is 0 whatever it holds.  An index
+// outside the vocabulary was met, or the list is empty.
+constexpr float kPoisoned = INFINITY;
 
 // Everything behind the sums of a row, by the G lanes that share it.  o: the sums over the whole row, or with
 // TAIL over the entries outside the list; first: bit i, this lane's entry i is the one of its index that counts
@@ -187,11 +189,15 @@ __device__ __forceinline__ void finish_row(i64 r, bool ok, int l, Online o, cons
             B = (Q + qr) * fast_exp2(to_all) - qr * fast_exp2(-(l2r + ms_slip(rest.m, c)));
         }
     }
-    bad = group_allreduce_i32<G, OpMaxI>(bad ? 1 : 0) != 0;
+    int seen = bad ? 2 : 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) seen |= e[i].at >= 0 ? 1 : 0;
+    seen = group_allreduce_i32<G, OpMaxI>(seen);  // 0: an empty list, 1: entries, 2 and more: an index out of range
+    bad = seen > 1;
     if (bad && a.status) raise_flag(a.status, CWR_FLAG_BAD_LABEL);
     if (!ok || l != 0) return;
-    a.loss[r] = bad ? __int_as_float(0x7fc00000) : loss / (float)(tp.inv * tp.inv);
-    if (a.stat) a.stat[r] = bad ? make_float4(0.f, 0.f, 0.f, kPoisoned) : make_float4(rest.m, B, o.m, l2);
+    a.loss[r] = bad ? __int_as_float(0x7fc00000) : seen == 0 ? 0.f : loss / (float)(tp.inv * tp.inv);
+    if (a.stat) a.stat[r] = seen != 1 ? make_float4(0.f, 0.f, 0.f, kPoisoned) : make_float4(rest.m, B, o.m, l2);
 }
 
 // G lanes per row (the row whole in registers), or one or NW waves per row that walk it in chunks.
@@ -396,7 +402,7 @@ __global__ __launch_bounds__(kWavesPerBlock * 64) void k_distill_grad(
     if (TAIL && st.x > -INFINITY) Q = fmaxf(Q, 1.f);  // with the tail's mass, where there is a tail
     const float c = tp.c;
     const Anchor ref = anchor(st.x, c);
-    const bool poisoned = st.w == kPoisoned;
+    const bool poisoned = st.w == kPoisoned;  // no gradient
     const float B = poisoned ? 0.f : st.y * gt;
     wave_sync();
     int place[E];

@@ -31,3 +31,36 @@ def test_shares_of_a_teacher_far_from_zero(V, K, base, T):
     dx, = torch.autograd.grad(loss.sum(), x)
     rel = EPS32 * (2 * slack + 3 * (math.log2(V + 1) + 126) + 2 * K)
     near(dx, d1, EPS32 * d1.abs() + 2 * tiny(torch.float32) + rel * scale, "dx")
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("V", [16, 41, 1024, 2500, 9000, 20000])
+def test_rows_without_a_list_do_not_count_whatever_is_in_them(V, tail):
+    """An empty list marks a row that is not to be learned from: loss 0 and gradient 0 exactly, also where the row holds
+    NaN, infinities or nothing, and the other rows' results stay what they are."""
+    gen = torch.Generator(device=DEV).manual_seed(V)
+    x = torch.randn((8, V), device=DEV, generator=gen)
+    top = torch.randn((8, 5), device=DEV, generator=gen).log_softmax(1) - 0.1
+    index = torch.stack([torch.randperm(V, device=DEV, generator=gen)[:5] for _ in range(8)]).to(torch.int32)
+    want_x = x.clone().requires_grad_(True)
+    want = pkg.distill_loss(want_x, top, index, tail=tail, reduction="none")
+    d_want, = torch.autograd.grad(want.sum(), want_x)
+    empty = torch.tensor([0, 1, 2, 3, 5, 6], device=DEV)
+    index[empty] = -1
+    x[1, V // 2] = math.nan
+    x[2] = math.nan
+    x[3, 0] = math.inf
+    x[5] = -math.inf
+    top[6] = math.nan  # what stands beside absent entries
+    kept = torch.tensor([4, 7], device=DEV)
+    x.requires_grad_(True)
+    rows = pkg.distill_loss(x, top, index, tail=tail, reduction="none")
+    assert (rows[empty] == 0).all() and torch.equal(rows[kept], want[kept])
+    d, = torch.autograd.grad(rows.sum(), x)
+    assert (d[empty] == 0).all() and torch.equal(d[kept], d_want[kept])
+    for reduction, part in (("sum", 1), ("mean", 8)):
+        loss = pkg.distill_loss(x, top, index, tail=tail, reduction=reduction)
+        exact = float(want[kept].double().sum()) / part
+        assert abs(float(loss) - exact) <= 2 * EPS32 * abs(exact)
+        d, = torch.autograd.grad(loss, x)
+        assert (d[empty] == 0).all() and torch.isfinite(d).all()
