@@ -305,7 +305,8 @@ class CompactJoiner(torch.nn.Module):
                                  blank, reduction, self.activation, total_rows=total_rows)
 
     def _row_scores(self, h, tokens, top_k, entropy, temperature):
-        if h.dtype in (torch.float16, torch.bfloat16) and h.size(1) % 32 == 0:
+        # under autocast the rows are of 16 bits and the weight is not: the logits are then those of forward()
+        if h.dtype in (torch.float16, torch.bfloat16) and self.out.weight.dtype == h.dtype and h.size(1) % 32 == 0:
             with torch.no_grad():
                 return joint_token_logprobs(h, self.out.weight, self.out.bias, tokens, top_k=top_k, entropy=entropy,
                                             temperature=temperature)
@@ -314,8 +315,8 @@ class CompactJoiner(torch.nn.Module):
     @torch.no_grad()
     def lattice_scores(self, enc_out, pred_out, lx, y, ly, blank: int = 0, top_k: int = 0, entropy: bool = False,
                        temperature: float = 1.0, total_rows: Optional[int] = None) -> TokenScores:
-        """Scores of every lattice cell without its logits (fp16 / bf16 modules; others go through stored
-        logits): logprobs (R, 2) of the blank and the cell's label (0 where a cell has no label), and on
+        """Scores of every lattice cell without its logits (fp16 / bf16 modules; others, autocast among them, go
+        through stored logits): logprobs (R, 2) of the blank and the cell's label (0 where a cell has no label), and on
         request the entropy and the top_k most probable entries, in the row order of forward().  A teacher's
         top_logprobs and top_index are what distill_loss(..., tail=True) takes.  No gradient."""
         if total_rows is None:
