@@ -308,8 +308,8 @@ class CompactJoiner(torch.nn.Module):
         # under autocast the rows are of 16 bits and the weight is not: the logits are then those of forward()
         if h.dtype in (torch.float16, torch.bfloat16) and self.out.weight.dtype == h.dtype and h.size(1) % 32 == 0:
             with torch.no_grad():
-                return joint_token_logprobs(h, self.out.weight, self.out.bias, tokens, top_k=top_k, entropy=entropy,
-                                            temperature=temperature)
+                return joint_token_logprobs(h, self.out.weight.contiguous(), self.out.bias, tokens, top_k=top_k,
+                                            entropy=entropy, temperature=temperature)
         return token_logprobs(self.out(h), tokens, top_k=top_k, entropy=entropy, temperature=temperature)
 
     @torch.no_grad()

@@ -35,3 +35,16 @@ def test_scores_under_autocast(half):
     assert float((s.logprobs.double() - ref["logprobs"]).abs().max()) <= tol
     assert torch.equal(s.top_index.long(), ref["top_index"])
     assert one.top_logprobs.shape == (3, 3) and torch.isfinite(one.top_logprobs).all()
+
+
+def test_scores_of_a_weight_that_is_a_transposed_view():
+    """An output layer tied to an embedding stored the other way round, as loss() takes it."""
+    j, lx, ly, y, e, p = setup(torch.bfloat16)
+    want = j.lattice_scores(e, p, lx, y, ly, top_k=4)
+    step = j.step_scores(e[:, 0], p[:, 0], top_k=3)
+    j.out.weight = torch.nn.Parameter(j.out.weight.detach().t().contiguous().t())
+    assert not j.out.weight.is_contiguous()
+    got = j.lattice_scores(e, p, lx, y, ly, top_k=4)
+    assert torch.equal(got.logprobs, want.logprobs) and torch.equal(got.top_index, want.top_index)
+    assert torch.equal(j.step_scores(e[:, 0], p[:, 0], top_k=3).top_logprobs, step.top_logprobs)
+    assert torch.isfinite(j.loss(e, p, lx, y, ly))
