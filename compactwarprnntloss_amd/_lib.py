@@ -76,6 +76,7 @@ SIGNATURES = {
     "cwr_distill_backward": (C.c_int, [_p, C.c_int, _i64, _i64, _i64, _p, _p, _i64, C.c_double, C.c_int, _p, _p, _i64,
                                        C.c_float, _p, _p]),
     "cwr_join": (C.c_int, [_p, _p, C.c_int, C.c_int, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _p, _p, _p]),
+    "cwr_join_rows": (C.c_int, [_p, _p, C.c_int, C.c_int, _i64, _i64, _p, _p]),
     "cwr_join_backward": (C.c_int, [_p, _p, C.c_int, C.c_int, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _p, _p, _p]),
 }
 

@@ -173,7 +173,7 @@ using namespace cwr;
 
 extern "C" {
 
-int cwr_version(void) { return 140; }
+int cwr_version(void) { return 141; }
 
 const char* cwr_strerror(int status) {
     switch (status) {
@@ -561,6 +561,17 @@ int cwr_join(const void* f, const void* g, int dtype, int act, int64_t N, int64_
     if (misaligned(f, es) || misaligned(g, es) || misaligned(h, es) || misaligned(status, 4)) return CWR_ERR_ALIGN;
     return launch_join(dtype, act, false, f, g, h, nullptr, lx, ly, reinterpret_cast<const i64*>(row_off), N, T_pad,
                        Up_pad, H, R, status, static_cast<hipStream_t>(stream));
+}
+
+int cwr_join_rows(const void* f, const void* g, int dtype, int act, int64_t R, int64_t H, void* h, void* stream) {
+    if (dtype < CWR_F32 || dtype > CWR_F64) return CWR_ERR_DTYPE;
+    if (act < CWR_ACT_NONE || act > CWR_ACT_RELU) return CWR_ERR_MODE;
+    if (R < 0 || H < 1) return CWR_ERR_SHAPE;
+    if (H > 0x3fffffff || R > 0xffffffffLL) return CWR_ERR_TOO_LARGE;
+    if (R > 0 && (!f || !g || !h)) return CWR_ERR_NULL;
+    const size_t es = elem_size(dtype);
+    if (misaligned(f, es) || misaligned(g, es) || misaligned(h, es)) return CWR_ERR_ALIGN;
+    return launch_join_rows(dtype, act, f, g, R * H, h, static_cast<hipStream_t>(stream));
 }
 
 int cwr_join_backward(const void* dh, const void* h, int dtype, int act, int64_t N, int64_t T_pad, int64_t Up_pad,

@@ -109,6 +109,9 @@ int launch_join(int dtype, int act, bool backward, const void* a, const void* b,
                 const int* ly, const i64* row_off, i64 N, i64 T_pad, i64 Up_pad, i64 H, i64 R, int* status,
                 hipStream_t stream);
 
+// one row of f and one of g per row of the output, n = rows x H elements
+int launch_join_rows(int dtype, int act, const void* f, const void* g, i64 n, void* out, hipStream_t stream);
+
 // Scores of rows of logits (scores.hip): pointers as in cwr_token_logprobs / cwr_token_logprobs_backward
 struct RowScores {
     const int* tokens;

@@ -147,6 +147,21 @@ __global__ __launch_bounds__(256) void k_join(const T* __restrict__ f, const T* 
     }
 }
 
+// One row of f and one of g per row of the output (a step of a search): no lattice to decode, n elements in all.
+// The output layer reads the rows next, so they stay in the caches.
+template <typename T, int VEC, int ACT>
+__global__ __launch_bounds__(256) void k_join_rows(const T* __restrict__ f, const T* __restrict__ g, i64 n,
+                                                   T* __restrict__ out) {
+    const i64 at = ((i64)blockIdx.x * 256 + threadIdx.x) * VEC;
+    if (at >= n) return;
+    const PackT<T, VEC> a = ld<T, VEC>(f + at), b = ld<T, VEC>(g + at);
+    PackT<T, VEC> o;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+        o.e[i] = Arith<T>::down(activate<ACT, T>(Arith<T>::up(a.e[i]) + Arith<T>::up(b.e[i])));
+    *reinterpret_cast<PackT<T, VEC>*>(out + at) = o;
+}
+
 // df: grid x = block of 256 packs, y = t, z = sequence.  One lane sums its columns over u; the rows
 // (t, 0..U) are contiguous in the compact layout.
 template <typename T, int VEC, int ACT>
@@ -306,6 +321,40 @@ int launch_join(int dtype, int act, bool backward, const void* a, const void* b,
         case CWR_F16: return join_typed<__half>(j, act, backward);
         case CWR_BF16: return join_typed<bf16_t>(j, act, backward);
         case CWR_F64: return join_typed<double>(j, act, backward);
+    }
+    return CWR_ERR_DTYPE;
+}
+
+template <typename T, int VEC>
+static int join_rows_act(const T* f, const T* g, i64 n, int act, T* out, hipStream_t stream) {
+    const i64 blocks = (n / VEC + 255) / 256;
+    if (blocks > (1 << 24) - 1) return CWR_ERR_TOO_LARGE;  // the runtime counts work-items in 32 bits
+    const dim3 grid((unsigned)blocks), block(256);
+    switch (act) {
+        case kActNone: CWR_LAUNCH((k_join_rows<T, VEC, kActNone>), grid, block, 0, stream, f, g, n, out); break;
+        case kActTanh: CWR_LAUNCH((k_join_rows<T, VEC, kActTanh>), grid, block, 0, stream, f, g, n, out); break;
+        case kActRelu: CWR_LAUNCH((k_join_rows<T, VEC, kActRelu>), grid, block, 0, stream, f, g, n, out); break;
+        default: return CWR_ERR_MODE;
+    }
+    return check_launch();
+}
+
+template <typename T>
+static int join_rows_typed(const void* f, const void* g, i64 n, int act, void* out, hipStream_t stream) {
+    const uintptr_t all = reinterpret_cast<uintptr_t>(f) | reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(out);
+    constexpr int VEC = Elem<T>::VEC;
+    const T *pf = static_cast<const T*>(f), *pg = static_cast<const T*>(g);
+    if (n % VEC == 0 && (all & 15u) == 0) return join_rows_act<T, VEC>(pf, pg, n, act, static_cast<T*>(out), stream);
+    return join_rows_act<T, 1>(pf, pg, n, act, static_cast<T*>(out), stream);
+}
+
+int launch_join_rows(int dtype, int act, const void* f, const void* g, i64 n, void* out, hipStream_t stream) {
+    if (n == 0) return CWR_OK;
+    switch (dtype) {
+        case CWR_F32: return join_rows_typed<float>(f, g, n, act, out, stream);
+        case CWR_F16: return join_rows_typed<__half>(f, g, n, act, out, stream);
+        case CWR_BF16: return join_rows_typed<bf16_t>(f, g, n, act, out, stream);
+        case CWR_F64: return join_rows_typed<double>(f, g, n, act, out, stream);
     }
     return CWR_ERR_DTYPE;
 }

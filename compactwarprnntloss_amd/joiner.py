@@ -15,7 +15,7 @@ import torch
 from . import _lib
 from .loss import (RESIDENT_JOINT_SIZES, _DTYPES, _offsets, _raise_on_flags, _raise_on_status, _stream_ptr,
                    joint_forward, joint_forward_fg)
-from .scores import TokenScores, joint_token_logprobs, lattice_tokens, token_logprobs
+from .scores import TokenScores, _call, joint_token_logprobs, lattice_tokens, token_logprobs
 
 _ACTS = {None: 0, "none": 0, "tanh": 1, "relu": 2}
 _DW_SPLIT = 16  # parts the rows of a block are cut into for the weight-gradient product
@@ -85,6 +85,23 @@ def compact_join(f: torch.Tensor, g: torch.Tensor, lx: torch.Tensor, ly: torch.T
     out = _Join.apply(f.contiguous(), g.contiguous(), lx, ly, int(total_rows), _ACTS[activation], row_off, status)
     if validate:
         _raise_on_status(status, "compact_join")
+    return out
+
+
+def _join_rows(f: torch.Tensor, g: torch.Tensor, activation: Optional[str]) -> torch.Tensor:
+    """act(f + g) row by row in compact_join's arithmetic (cwr_join_rows); no gradient."""
+    if activation not in _ACTS:
+        raise RuntimeError(f"activation must be one of {sorted(k for k in _ACTS if k)} or None")
+    if f.shape != g.shape:  # one frame and several hypotheses, or the other way round
+        f, g = torch.broadcast_tensors(f, g)
+    if f.dim() != 2 or f.dtype != g.dtype or f.dtype not in _DTYPES:
+        raise RuntimeError("f and g must be (B, H) of one supported dtype")
+    if not f.is_cuda or f.device != g.device:
+        raise RuntimeError("f and g must be CUDA tensors on one device")
+    f, g = f.contiguous(), g.contiguous()
+    out = torch.empty_like(f)
+    _call("cwr_join_rows", f.device, f.data_ptr(), g.data_ptr(), _DTYPES[f.dtype], _ACTS[activation], f.size(0),
+          f.size(1), out.data_ptr())
     return out
 
 
@@ -329,7 +346,7 @@ class CompactJoiner(torch.nn.Module):
     def step_scores(self, enc_frame, pred_state, tokens: Optional[torch.Tensor] = None, top_k: int = 1,
                     entropy: bool = False, temperature: float = 1.0) -> TokenScores:
         """One step of a search: row b scores act(enc(enc_frame[b]) + pred(pred_state[b])), (B, enc_dim) and
-        (B, pred_dim), e.g. one row per hypothesis.  tokens (B,) or (B, M) int32 or None.  No gradient."""
-        z = self.enc(enc_frame) + self.pred(pred_state)
-        h = torch.tanh(z) if self.activation == "tanh" else torch.relu(z) if self.activation == "relu" else z
+        (B, pred_dim), e.g. one row per hypothesis, with the joint rows of lattice_scores bit for bit.  tokens (B,)
+        or (B, M) int32 or None.  No gradient."""
+        h = _join_rows(self.enc(enc_frame), self.pred(pred_state), self.activation)
         return self._row_scores(h, tokens, top_k, entropy, temperature)

@@ -269,6 +269,11 @@ int cwr_join(const void* f, const void* g, int dtype, int act, int64_t N, int64_
              const int32_t* lx, const int32_t* ly, const int64_t* row_off, int64_t R, void* h, int32_t* status,
              void* stream);
 
+/* One step of a search: h[r, :] = act(f[r, :] + g[r, :]) for R rows that each have a frame and a predictor state of
+ * their own, in cwr_join's arithmetic (a row has the bits it has in the lattice).
+ *   f, g, h (R, H) contiguous;  act a cwr_activation.  No backward pass. */
+int cwr_join_rows(const void* f, const void* g, int dtype, int act, int64_t R, int64_t H, void* h, void* stream);
+
 /* Backward of cwr_join: df[n, t, :] = sum over u of dz, dg[n, u, :] = sum over t of dz, where
  * dz = dh * act'(z) with act' taken from the stored output h (unused, may be NULL, for
  * CWR_ACT_NONE).  Sums run in a fixed order (no atomics); every element of df and dg is written,

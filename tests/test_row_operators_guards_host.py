@@ -1,9 +1,10 @@
-"""What is checked of the row operators without a GPU: the device assembly."""
+"""What is checked of the row operators without a GPU: the device assembly, refusals."""
 import glob
 import os
 
 import pytest
 
+from compactwarprnntloss_amd import _lib
 from compactwarprnntloss_amd.build import HERE, early_scalar_reads
 
 
@@ -27,3 +28,17 @@ def test_no_kernel_reads_a_scalar_register_too_soon():
     for path in listings:
         with open(path) as f:
             assert early_scalar_reads(f.read()) == [], os.path.basename(path)
+
+
+def test_checks_of_the_step_rows():
+    """cwr_join_rows(f, g, dtype, act, R, H, h, stream): refused before any HIP call."""
+    call = _lib.load().cwr_join_rows
+    p = [0x10000 * n for n in range(1, 4)]
+    null, dtype, mode, shape, align, large = 1, 2, 3, 4, 6, 8
+    assert call(None, p[1], 0, 0, 5, 8, p[2], None) == null and call(p[0], None, 0, 0, 5, 8, p[2], None) == null
+    assert call(p[0], p[1], 0, 0, 5, 8, None, None) == null
+    assert call(p[0], p[1], 4, 0, 5, 8, p[2], None) == dtype and call(p[0], p[1], 0, 3, 5, 8, p[2], None) == mode
+    assert call(p[0], p[1], 0, 0, -1, 8, p[2], None) == shape and call(p[0], p[1], 0, 0, 5, 0, p[2], None) == shape
+    assert call(p[0] + 2, p[1], 0, 0, 5, 8, p[2], None) == align and call(p[0], p[1], 1, 0, 5, 8, p[2] + 1, None) == align
+    assert call(p[0], p[1], 0, 0, 5, 1 << 30, p[2], None) == large and call(p[0], p[1], 0, 0, 1 << 33, 8, p[2], None) == large
+    assert call(None, None, 0, 0, 0, 8, None, None) == 0
