@@ -329,6 +329,8 @@ def lattice_tokens(lx: torch.Tensor, y: torch.Tensor, ly: torch.Tensor, total_ro
     for name, t in (("lx", lx), ("y", y), ("ly", ly)):
         if not t.is_cuda or t.dtype != torch.int32 or not t.is_contiguous():
             raise RuntimeError(f"{name} must be a contiguous CUDA int32 tensor")
+        if t.device != lx.device:
+            raise RuntimeError(f"{name} must be on the device of lx")
     if lx.dim() != 1 or lx.shape != ly.shape or y.dim() not in (1, 2) or (y.dim() == 2 and y.size(0) != lx.size(0)):
         raise RuntimeError("lx, ly must be (N,), y (N, U) or concatenated")
     assert blank >= 0 and blank < V

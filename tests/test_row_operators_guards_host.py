@@ -3,7 +3,9 @@ import glob
 import os
 
 import pytest
+import torch
 
+import compactwarprnntloss_amd as pkg
 from compactwarprnntloss_amd import _lib
 from compactwarprnntloss_amd.build import HERE, early_scalar_reads
 
@@ -42,3 +44,26 @@ def test_checks_of_the_step_rows():
     assert call(p[0] + 2, p[1], 0, 0, 5, 8, p[2], None) == align and call(p[0], p[1], 1, 0, 5, 8, p[2] + 1, None) == align
     assert call(p[0], p[1], 0, 0, 5, 1 << 30, p[2], None) == large and call(p[0], p[1], 0, 0, 1 << 33, 8, p[2], None) == large
     assert call(None, None, 0, 0, 0, 8, None, None) == 0
+
+
+def test_lattice_tokens_refuses_tensors_of_several_devices():
+    """A kernel on one device would read another's memory.  The checks look at a tensor's description only, so that
+    stand-ins do where there is one device or none."""
+    class Described:
+        is_cuda, dtype = True, torch.int32
+
+        def __init__(self, index, *shape):
+            self.device, self.shape = torch.device("cuda", index), torch.Size(shape)
+
+        def is_contiguous(self):
+            return True
+
+        def dim(self):
+            return len(self.shape)
+
+        def size(self, d):
+            return self.shape[d]
+    for devices in ((0, 1, 0), (0, 0, 1), (1, 0, 0)):
+        lx, y, ly = (Described(i, *shape) for i, shape in zip(devices, ((2,), (2, 3), (2,))))
+        with pytest.raises(RuntimeError, match="device of lx"):
+            pkg.lattice_tokens(lx, y, ly, 4, 8)
