@@ -245,3 +245,23 @@ def test_distillation_at_small_temperatures(V, T, tail):
     dx, = torch.autograd.grad(loss.sum(), x)
     rel = EPS32 * (2 * slack_of(V) + 3 * (math.log2(V + 1) + 126) + 6)
     near(dx, d1, EPS32 * d1.abs() + 2 * tiny(torch.float32) + rel * scale, "dx")
+
+
+@pytest.mark.parametrize("level", [-1e9, -1e10, -1e30])
+@pytest.mark.parametrize("R,V", [(40, 200), (30, 2500), (3000, 1300), (13000, 1100)])
+def test_joint_scores_with_a_vocabulary_masked_by_the_bias(R, V, level):
+    """Entries whose bias is a finite constant, a whole chunk of them among others: sums of products vanish beside it,
+    and what is left is the rest of the vocabulary."""
+    from tests.test_joint_scores_gpu import grid_problem
+    h, w, b, z, gen = grid_problem(R, V, 128, torch.bfloat16, seed=V, bias="f32")
+    cut = min(1024, V // 2)
+    b[:cut] = level
+    tok = torch.randint(cut, V, (R, 2), device=DEV, generator=gen, dtype=torch.int32)
+    z[:, :cut] = -math.inf
+    ref = scores_ref(z, tok, 5, 1.0)
+    out = pkg.joint_token_logprobs(h, w, b, tok, top_k=5, entropy=True)
+    slack = EPS32 * slack_of(V)
+    assert torch.equal(out.top_index.long(), ref["top_index"])
+    near(out.lse, ref["lse"], slack + EPS32 * ref["lse"].abs(), "lse")
+    near(out.logprobs, ref["logprobs"], slack + EPS32 * ref["logprobs"].abs(), "logprobs")
+    near(out.entropy, ref["entropy"], slack * (2 + 2 * math.log2(V + 1)) + EPS32 * ref["entropy"].abs(), "entropy")
