@@ -207,8 +207,13 @@ __global__ __launch_bounds__(256) void k_logits_tile(const T* __restrict__ h, co
 }
 
 // X(ND, H / 16, NMV, WAVES, RK, workgroups per CU, two register sets of weight loads in flight): the shapes of
-// the fused output layer's forward pass, at H = 512 with two sets: loads issued behind a tile's stores return
-// behind them, and a slice more of lead hides part of that (62464 x 1024: 95 -> 89 us)
+// the fused output layer's forward pass, at H = 512 with two sets (loads issued behind a tile's stores return
+// behind them, and a slice more of lead hides part of that: 62464 x 1024 took 95 -> 89 us on one box, 79 either way on
+// another).  The flag here / the other way round, us, 62464 x 1024: H = 128 46 / 46, 192 48 / 70, 256 54 / 54, 320 62 / 88,
+// 384 65 / 68, 448 74 / 102, 512 78 / 79, 576 93 / 126, 640 104 / 110, 704 135 / 262, 768 137 / 144, 832 150 / 425,
+// 896 151 / 161, 960 170 / 498, 1024 166 / 175 (with an odd number of slices a tile the two sets take turns from tile
+// to tile as well, and which is which is known at run time only).  H = 576 and 640 spill 6 and 28 registers and are still
+// ahead of the streamed walk: 93 against 136 and 104 against 146 us (H = 128 46 / 65, 512 79 / 130, 1024 166 / 213).
 #define CWR_LOGIT_SHAPES(X) X(1, 8, 4, 8, 64, 1, true) X(1, 12, 4, 8, 64, 1, false) X(1, 16, 4, 8, 64, 1, true) \
                             X(1, 20, 4, 8, 64, 1, false) X(1, 24, 4, 8, 64, 1, true) X(1, 28, 4, 8, 64, 1, false) \
                             X(1, 32, 4, 8, 64, 1, true) X(1, 36, 4, 8, 64, 1, false) X(1, 40, 4, 8, 64, 1, false) \
@@ -229,9 +234,13 @@ static int split_vocabulary(i64 row_blocks, i64 resident, int V, unsigned* split
 template <typename T, typename TB>
 static int logits_typed(const T* h, const T* w, const TB* bias, i64 R, int H, int V, int pitch, float* out,
                         hipStream_t stream) {
-    // By the size of the product (us, few / tiled / walked; bf16): 256 x 1024, H = 512: 4.8 / 6.6 / 17;
-    // 128 x 4096, H = 640: 8.9 / 7.7 / 18;  4096 x 1024: 36 / 15 / 25;  2048 x 4096: 97 / 28 / 30;
-    // 16384 x 1024: 132 / 44 / 34;  4096 x 4096: 187 / 49 / 44.
+    // By the number of logits, which moves both borders little with the joint size (us, few / tiled / walked; bf16):
+    //   V = 1024          R * V = 0.2e6       0.4e6            1.6e6             6e6                12e6
+    //     H = 128       4.8 / 4.6 / 8.0   5.3 / 4.7 / 8.0   12 / 6.7 / 9.8   32 / 18.3 / 13.1   52 / 17 / 15
+    //     H = 512       5.2 / 6.7 / 15    6.9 / 6.8 / 16    18 / 9.5 / 18    49 / 18.3 / 19.4   94 / 32 / 27
+    //     H = 1024      6.7 / 9.1 / 18    10 / 9.6 / 18     29 / 15 / 19     90 / 30 / 30      175 / 52 / 49
+    //   V = 4096, H = 640 5.9 / 7.2 / 16  8.6 / 7.2 / 17    24 / 10.5 / 22   71 / 21 / 25      137 / 37 / 37
+    //   V = 300, H = 1056 5.8 / 9.7 / 31  9.1 / 10 / 32     36 / 17 / 37    125 / 42 / 41      240 / 80 / 50 (streamed)
     if (R * V <= 400000) {
         CWR_LAUNCH((k_logits_few<T, TB>), dim3((unsigned)((V + 31) / 32), (unsigned)((R + 31) / 32)), dim3(64 * kFewWaves),
                    0, stream, h, w, bias, R, H, V, pitch, out);

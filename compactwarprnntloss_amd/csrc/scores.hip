@@ -570,7 +570,10 @@ static int scores_typed(const T* x, i64 R, int V, i64 stride, const Temper& tp, 
     const int span = V + (EDGE ? RowPacks<T>::VEC - 1 : 0);  // places a row can take on the pack grid
     int G = 4;
     while (G < 64 && G * kLaneElems < span) G *= 2;
-    // striking out costs K rounds of every 64 / G rows, the list a fixed price per row
+    // Striking out costs K rounds of every 64 / G rows, the list a fixed price per row and more from some 20
+    // alternatives on, where its bound lets many in.  us per 200000 fp32 rows, struck out / listed: V = 64 (G = 4) K = 4
+    // 19 / 160, K = 64 141 / 360; V = 128 (8) K = 40 172 / 479, K = 64 264 / 606; V = 256 (16) K = 20 186 / 190, K = 32
+    // 277 / 207; V = 512 (32) K = 4 121 / 147, K = 8 180 / 156, K = 10 211 / 160, K = 16 301 / 170; bf16 alike.
     if (G < 64 && a.K * G > 320) G = 64;
 #define CWR_GROUP(GG)                                                                                              \
     if (G == GG) {                                                                                                 \

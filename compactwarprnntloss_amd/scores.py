@@ -152,8 +152,8 @@ def token_logprobs(x: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, to
                    temperature: float = 1.0, validate: bool = False) -> TokenScores:
     """Scores of the rows of logits x under softmax(x / temperature).
 
-    x         (R, V) fp32, fp16, bf16 or fp64 logits (or log-probabilities); the entries of a row adjacent,
-              rows any distance apart (a slice of a padded tensor is fine)
+    x         (R, V) fp32, fp16, bf16 or fp64 logits (or log-probabilities), fp64 rounded to fp32 when read; the
+              entries of a row adjacent, rows any distance apart (a slice of a padded tensor is fine)
     tokens    (R,) or (R, M) int32, M <= 64: entries to score; -1 stands for no token (0, no gradient)
     top_k     number of most probable entries to return, <= 64, in descending order, equal ones by ascending
               index (NaN ranks with -inf)
@@ -279,7 +279,7 @@ def distill_loss(x: torch.Tensor, top_logits: torch.Tensor, top_index: torch.Ten
 
     x           (R, V) student logits, as for token_logprobs
     top_logits  (R, K) the teacher's values, top_index (R, K) int32 the entries they belong to, K <= 64;
-                an index of -1 is absent, a row whose list is empty has loss 0 and gradient 0
+                an index of -1 is absent, a row whose list is empty has loss 0 and gradient 0 whatever x holds
     tail        False: the teacher is softmax(top_logits / temperature) over the list.
                 True: top_logits are log-probabilities at this temperature (token_logprobs(...,
                 temperature=temperature).top_logprobs); the mass they leave is one more class, compared

@@ -398,7 +398,7 @@ int cwr_joint_token_logprobs(const void* h, const void* w, const void* bias, int
  *             not listed:  loss[r] = temperature^2 * (sum_k q_k (log q_k - log p[i_k]) + q_r (log q_r - log p_r)).
  *             A row whose unlisted entries are none, or all -inf, has no such class (no q_r term).
  * With the list (blank, label) and a tail this is the three-class distillation of a lattice cell.
- * A row whose list is empty (all absent) has loss 0 and gradient 0.  A listed entry with x = -inf makes the
+ * A row whose list is empty (all absent) has loss 0 and gradient 0, whatever x holds in it.  A listed entry with x = -inf makes the
  * loss infinite; the gradient takes its p as 0.  An index listed twice counts each
  * time, and once for what is not listed.  An index below -1 or >= V: loss NaN, gradient 0,
  * CWR_FLAG_BAD_LABEL.  The reference has no counterpart.
