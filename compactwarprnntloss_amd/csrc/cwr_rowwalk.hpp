@@ -20,6 +20,7 @@ constexpr int kLaneElems = 16;  // elements a lane holds of a chunk
 struct Temper {
     float c;     // log2(e) / T
     double inv;  // 1 / T
+    double sq;   // T^2
 };
 
 template <typename T> struct RowPacks {
@@ -320,6 +321,7 @@ inline Temper make_temper(double temperature) {
     Temper tp;
     tp.c = (float)(1.4426950408889634 / temperature);
     tp.inv = 1.0 / temperature;
+    tp.sq = temperature * temperature;
     return tp;
 }
 

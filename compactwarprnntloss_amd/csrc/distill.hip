@@ -163,10 +163,12 @@ __device__ __forceinline__ void finish_row(i64 r, bool ok, int l, Online o, cons
     // taken in 64 bits (an error of the row's sum itself cancels, the shares being nearly those of the teacher).
     const double l2d = empty ? 0.0 : log2_f64(o.s) - (double)ms_slip(o.m, c);
     const float l2 = (float)l2d;
+    // A term is rounded to fp32 once, as it enters the sum: log p of a listed entry masked with the lowest value of its
+    // type is beyond fp32 where T < 1, T^2 log p where T > 1, and q T^2 log p is neither
     float loss = 0.f;
 #pragma unroll
     for (int i = 0; i < E; ++i)
-        loss += q[i] == 0.f || e[i].at < 0 ? 0.f : q[i] * (float)((double)logq[i] - logprob_f64(e[i].x, o.m, l2d, tp));
+        loss += q[i] == 0.f || e[i].at < 0 ? 0.f : (float)((double)q[i] * ((double)logq[i] - logprob_f64(e[i].x, o.m, l2d, tp)) * tp.sq);
     loss = row_sum<G>(loss);
     float B = empty ? 0.f : Q * fast_exp2(-(l2 + ms_slip(o.m, c)));
     if (TAIL) {
@@ -183,7 +185,7 @@ __device__ __forceinline__ void finish_row(i64 r, bool ok, int l, Online o, cons
             const float l2r = (float)l2rd;
             if (qr > 0.f) {
                 const double logpr = ((double)rest.m - (double)o.m) * tp.inv + (l2rd - l2d) * 0.6931471805599453;
-                loss += qr * (float)(log2_f64(qr) * 0.6931471805599453 - logpr);
+                loss += (float)((double)qr * (log2_f64(qr) * 0.6931471805599453 - logpr) * tp.sq);
             }
             const float to_all = anchor_shift(rest.m, o.m, c) - (l2 + ms_slip(o.m, c));
             B = (Q + qr) * fast_exp2(to_all) - qr * fast_exp2(-(l2r + ms_slip(rest.m, c)));
@@ -196,7 +198,7 @@ __device__ __forceinline__ void finish_row(i64 r, bool ok, int l, Online o, cons
     bad = seen > 1;
     if (bad && a.status) raise_flag(a.status, CWR_FLAG_BAD_LABEL);
     if (!ok || l != 0) return;
-    a.loss[r] = bad ? __int_as_float(0x7fc00000) : seen == 0 ? 0.f : loss / (float)(tp.inv * tp.inv);
+    a.loss[r] = bad ? __int_as_float(0x7fc00000) : seen == 0 ? 0.f : loss;
     if (a.stat) a.stat[r] = seen != 1 ? make_float4(0.f, 0.f, 0.f, kPoisoned) : make_float4(rest.m, B, o.m, l2);
 }
 
